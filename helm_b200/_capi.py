@@ -18,7 +18,7 @@ from . import build as _build
 
 HELM_OK = 0
 DTYPE_FP32, DTYPE_FP16, DTYPE_BF16 = 0, 1, 2
-DEV_TIMEOUT, DEV_BAD_PAGE = 1, 2
+DEV_TIMEOUT, DEV_BAD_PAGE, DEV_NO_PAGES = 1, 2, 4
 
 _TORCH_TO_HELM = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16,
                   torch.bfloat16: DTYPE_BF16}
@@ -82,6 +82,29 @@ _SIGNATURES = {
     "helm_ipc_close": (_I, [_P]),
     "helm_seq_exchange_merge": (_I, [_P, _I, _I, _P, _P, _I64, _I, _P, _I, _P,
                                      ctypes.c_uint64, _P]),
+    "helm_fp4_page_bytes": (_I64, [_I, _I, _I]),
+    "helm_kv_append_fp4": (_I, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,   # q, k, v
+        _P, _P, _F,                                       # norm weights, eps
+        _P, _P, _I64,                                     # cos, sin, stride
+        _P, _I64, _I64,                                   # q_out
+        _P, _I64, _P,                                     # pool, pool_pages, slot_rows
+        _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "helm_gather_kv_rows_fp4": (_I, [_P, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _I,
+                                     _I, _F, _F, _P]),
+    "helm_paged_decode_fp4_workspace_bytes": (_I64, [_I, _I, _I, _I]),
+    "helm_paged_decode_attention_fp4": (_I, [
+        _P, _I64, _I64,            # q, strides
+        _P, _I64,                  # pool, pool_pages
+        _P, _I64, _I, _P,          # page_table, pt_stride_b, max_pages, kv_lens
+        _P, _I, _I64,              # mask, mask_dtype, mask_stride_b
+        _P, _I64, _I64, _P,        # out, strides, lse
+        _P, _I64,                  # workspace, bytes
+        _I, _I, _I, _I, _I, _I,    # batch, hq, hkv, head_dim, page_size, dtype
+        _F, _F, _F, _F, _I, _P]),  # scale, softcap, k_scale, v_scale, hint, stream
+    "helm_build_step_tables": (_I, [_P, _P, _P, _I64, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I,
+                                    _I, _I, _P]),
+    "helm_sample_tokens": (_I, [_P, _I64, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
 }
 
 _lib = None
@@ -616,3 +639,281 @@ def gemv_max_batch(k: int, elem: int = 2) -> int:
         if (nb * stride * elem + 127) // 128 * 128 + nw + threads * ring + static <= 224 * 1024:
             return nb
     raise HelmError(f"input width {k} too large for decode_gemv")
+
+
+# ── 4-bit pages ───────────────────────────────────────────────────────────────
+def fp4_pool(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
+             device) -> torch.Tensor:
+    """A zeroed pool of 4-bit pages, uint8 [num_pages, Hkv, page_size / 16,
+    18 * head_dim] (include/helm_b200.h gives the format)."""
+    fp4_page_bytes(num_kv_heads, page_size, head_dim)  # refuses unsupported shapes
+    return torch.zeros(num_pages, num_kv_heads, page_size // 16, 18 * head_dim, dtype=torch.uint8,
+                       device=device)
+
+
+def fp4_page_bytes(num_kv_heads: int, page_size: int, head_dim: int) -> int:
+    """Bytes of a 4-bit page (K and V of all KV heads)."""
+    n = int(lib().helm_fp4_page_bytes(num_kv_heads, page_size, head_dim))
+    if n < 0:
+        raise HelmError(f"unsupported 4-bit page: {num_kv_heads} KV heads, page_size {page_size} "
+                        f"(a multiple of 16), head_dim {head_dim} (64, 128 or 256)")
+    return n
+
+
+def _check_fp4_pool(what: str, pool: torch.Tensor, hkv: int, page_size: int, d: int, dev) -> None:
+    if (pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[1] != hkv
+            or pool.shape[2] * 16 != page_size or pool.shape[3] != 18 * d
+            or not pool.is_contiguous() or pool.device != dev):
+        raise HelmError(f"{what}: pool must be a contiguous uint8 [pages, Hkv, page_size / 16, "
+                        f"18 * head_dim] tensor on {dev}")
+
+
+def _on(what: str, dev, **tensors) -> None:
+    """Every given tensor lives on the CUDA device `dev`."""
+    if dev.type != "cuda":
+        raise HelmError(f"{what} runs on CUDA tensors only")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise HelmError(f"{what}: {name} is on {t.device}, not on {dev}")
+
+
+def kv_append_fp4(*, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor,
+                  slot_rows: torch.Tensor, page_size: int, q: Optional[torch.Tensor] = None,
+                  q_out: Optional[torch.Tensor] = None, q_norm_w: Optional[torch.Tensor] = None,
+                  k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                  k_scale: float = 1.0, v_scale: float = 1.0, stream=None) -> None:
+    """kv_append into 4-bit pages: (QK-RMSNorm, RoPE, quantising page write),
+    fp32 throughout.  q [N, Hq, D], k/v [N, Hkv, D] (unit dim stride, 16-byte
+    aligned rows), cos/sin [N, D], slot_rows int64 [N] (-1 = skip; distinct),
+    pool from fp4_pool, k_scale/v_scale the cache's scales (powers of two)."""
+    N, Hkv, D = k.shape
+    dev = k.device
+    _on("kv_append_fp4", dev, v=v, q=q, q_out=q_out, cos=cos, sin=sin, q_norm_w=q_norm_w,
+        k_norm_w=k_norm_w, slot_rows=slot_rows)
+    _check_fp4_pool("kv_append_fp4", pool, Hkv, page_size, D, dev)
+    if v.shape != k.shape or v.stride(2) != 1 or k.stride(2) != 1:
+        raise HelmError("kv_append_fp4: k and v must be [N, Hkv, D] with a unit dim stride")
+    if (q is None) != (q_out is None):
+        raise HelmError("kv_append_fp4: q and q_out go together")
+    if q is not None and (q.shape[0] != N or q.shape[2] != D or q_out.shape != q.shape
+                          or q.stride(2) != 1 or q_out.stride(2) != 1):
+        raise HelmError("kv_append_fp4: q and q_out must be [N, Hq, D] with a unit dim stride")
+    if (cos is None) != (sin is None):
+        raise HelmError("kv_append_fp4: cos and sin go together")
+    if cos is not None and (cos.shape != (N, D) or sin.shape != (N, D) or cos.stride(1) != 1
+                            or sin.stride() != cos.stride()):
+        raise HelmError("kv_append_fp4: cos and sin must be [N, D] with equal strides")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            raise HelmError("kv_append_fp4: norm weights must be contiguous [D]")
+    dt = k.dtype
+    for t in (v, q, q_out, q_norm_w, k_norm_w, cos, sin):
+        if t is not None and t.dtype != dt:
+            raise HelmError(f"kv_append_fp4: {t.dtype} where {dt} is used")
+    if slot_rows.dtype != torch.int64 or slot_rows.shape != (N,) or not slot_rows.is_contiguous():
+        raise HelmError("kv_append_fp4: slot_rows must be contiguous int64 [N]")
+    with _on_device(dev):
+        rc = lib().helm_kv_append_fp4(
+            _ptr(q), q.stride(0) if q is not None else 0, q.stride(1) if q is not None else 0,
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            _ptr(q_norm_w), _ptr(k_norm_w), eps,
+            _ptr(cos), _ptr(sin), cos.stride(0) if cos is not None else 0,
+            _ptr(q_out), q_out.stride(0) if q is not None else 0,
+            q_out.stride(1) if q is not None else 0,
+            pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(), N,
+            q.shape[1] if q is not None else 0, Hkv, D, page_size, helm_dtype(dt),
+            k_scale, v_scale, _stream_handle(dev, stream))
+    _check(rc, "helm_kv_append_fp4")
+
+
+def gather_kv_rows_fp4(pool: torch.Tensor, slot_rows: torch.Tensor, *, page_size: int,
+                       dtype: torch.dtype, k_scale: float = 1.0, v_scale: float = 1.0,
+                       k_out: Optional[torch.Tensor] = None,
+                       v_out: Optional[torch.Tensor] = None, stream=None):
+    """K, V [N, Hkv, D] in `dtype`: the values of the pool rows slot_rows
+    (int64 [N]; a negative row gives zeros).  k_out / v_out may be strided."""
+    dev = pool.device
+    _on("gather_kv_rows_fp4", dev, slot_rows=slot_rows, k_out=k_out, v_out=v_out)
+    if pool.dim() != 4 or pool.shape[3] % 18:
+        raise HelmError("gather_kv_rows_fp4: pool is not a pool of 4-bit pages")
+    Hkv, D = pool.shape[1], pool.shape[3] // 18
+    _check_fp4_pool("gather_kv_rows_fp4", pool, Hkv, page_size, D, dev)
+    if slot_rows.dtype != torch.int64 or slot_rows.dim() != 1 or not slot_rows.is_contiguous():
+        raise HelmError("gather_kv_rows_fp4: slot_rows must be contiguous int64 [N]")
+    shape = (slot_rows.shape[0], Hkv, D)
+    with _on_device(dev):
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=dtype, device=dev)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=dtype, device=dev)
+        for t in (k_out, v_out):
+            if t.shape != shape or t.dtype != dtype or t.stride(2) != 1:
+                raise HelmError("gather_kv_rows_fp4: outputs must be [N, Hkv, D] in dtype with a "
+                                "unit dim stride")
+        rc = lib().helm_gather_kv_rows_fp4(
+            pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(), k_out.data_ptr(),
+            k_out.stride(0), k_out.stride(1), v_out.data_ptr(), v_out.stride(0), v_out.stride(1),
+            shape[0], Hkv, D, page_size, helm_dtype(dtype), k_scale, v_scale,
+            _stream_handle(dev, stream))
+    _check(rc, "helm_gather_kv_rows_fp4")
+    return k_out, v_out
+
+
+_fp4_ws_bytes: dict = {}
+
+
+def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
+                               kv_lens: torch.Tensor, *, num_kv_heads: int, page_size: int,
+                               scale: float, softcap: Optional[float] = None,
+                               mask: Optional[torch.Tensor] = None, k_scale: float = 1.0,
+                               v_scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                               lse: Optional[torch.Tensor] = None, max_kv_len_hint: int = 0,
+                               stream=None):
+    """Decode attention over a pool of 4-bit pages (fp4_pool).
+
+    q [B, Hq, D] (dim stride 1); page_table int32 [B, max_pages]; kv_lens int32
+    [B]; mask additive [B or 1, T] with T >= max(kv_lens), -inf excludes a key.
+    Returns (out [B, Hq, D] in q.dtype, lse fp32 [B, Hq] or None).
+    """
+    dev = q.device
+    _on("paged_decode_attention_fp4", dev, page_table=page_table, kv_lens=kv_lens, mask=mask,
+        out=out, lse=lse)
+    B, Hq, D = q.shape
+    _check_fp4_pool("paged_decode_attention_fp4", pool, num_kv_heads, page_size, D, dev)
+    if q.stride(2) != 1:
+        raise HelmError("q must have a unit stride on the head dim")
+    if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32:
+        raise HelmError("page_table and kv_lens must be int32")
+    if (page_table.dim() != 2 or page_table.shape[0] != B or page_table.stride(1) != 1
+            or kv_lens.shape != (B,) or not kv_lens.is_contiguous()):
+        raise HelmError("page_table must be [B, max_pages] with contiguous rows, kv_lens [B]")
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:
+        raise HelmError("out must be [B, Hq, D] in the query dtype, unit dim stride")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq)
+                            or not lse.is_contiguous()):
+        raise HelmError("lse must be contiguous fp32 [B, Hq]")
+    mask_ptr, mask_dt, mask_sb = None, 0, 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] not in (1, B):
+            raise HelmError("mask must be [B or 1, T]")
+        if mask.stride(1) != 1:
+            mask = mask.contiguous()
+        mask_ptr, mask_dt = mask.data_ptr(), helm_dtype(mask.dtype)
+        mask_sb = mask.stride(0) if mask.shape[0] > 1 else 0
+    key = (dev.index, B, Hq, num_kv_heads, D)
+    with _on_device(dev):
+        nbytes = _fp4_ws_bytes.get(key)
+        if nbytes is None:
+            nbytes = _fp4_ws_bytes[key] = int(
+                lib().helm_paged_decode_fp4_workspace_bytes(B, Hq, num_kv_heads, D))
+        # scratch of this call alone: two captured graphs, or two streams, share none
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        if stream is not None:
+            ws.record_stream(stream)
+        rc = lib().helm_paged_decode_attention_fp4(
+            q.data_ptr(), q.stride(0), q.stride(1), pool.data_ptr(), pool.shape[0],
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(),
+            mask_ptr, mask_dt, mask_sb, out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
+            ws.data_ptr(), nbytes, B, Hq, num_kv_heads, D, page_size, helm_dtype(q.dtype), scale,
+            softcap or 0.0, k_scale, v_scale, max_kv_len_hint, _stream_handle(dev, stream))
+    _check(rc, "helm_paged_decode_attention_fp4")
+    return out, lse
+
+
+# ── the step of a continuous batch ────────────────────────────────────────────
+def build_step_tables(past_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.Tensor,
+                      free_pages: torch.Tensor, free_count: torch.Tensor, *, page_size: int,
+                      num_rows: int, free_count_out: Optional[torch.Tensor] = None,
+                      kv_lens: Optional[torch.Tensor] = None,
+                      cu_tokens: Optional[torch.Tensor] = None,
+                      seq_ids: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None,
+                      slot_rows: Optional[torch.Tensor] = None, stream=None):
+    """Page tables, slot rows and positions of one step from the requests' lengths.
+
+    past_lens, new_lens int32 [B] (new < 0: the request leaves); page_table
+    int32 [B, max_pages], free_pages int32 [capacity] and free_count int32 [1]
+    (updated in place; the count goes to free_count_out when given).  num_rows:
+    token rows written (>= the step's tokens; the rest get slot_rows -1).
+    Returns (kv_lens [B], cu_tokens [B + 1], seq_ids, positions int32 [num_rows],
+    slot_rows int64 [num_rows]); kv_lens may be past_lens itself.
+    """
+    dev = past_lens.device
+    _on("build_step_tables", dev, new_lens=new_lens, page_table=page_table, free_pages=free_pages,
+        free_count=free_count, free_count_out=free_count_out, kv_lens=kv_lens,
+        cu_tokens=cu_tokens, seq_ids=seq_ids, positions=positions, slot_rows=slot_rows)
+    B = past_lens.shape[0]
+    i32 = torch.int32
+    if free_count_out is None:
+        free_count_out = free_count
+    if kv_lens is None:
+        kv_lens = torch.empty(B, dtype=i32, device=dev)
+    if cu_tokens is None:
+        cu_tokens = torch.empty(B + 1, dtype=i32, device=dev)
+    if seq_ids is None:
+        seq_ids = torch.empty(num_rows, dtype=i32, device=dev)
+    if positions is None:
+        positions = torch.empty(num_rows, dtype=i32, device=dev)
+    if slot_rows is None:
+        slot_rows = torch.empty(num_rows, dtype=torch.int64, device=dev)
+    for name, t, n, dt in (("past_lens", past_lens, B, i32), ("new_lens", new_lens, B, i32),
+                           ("free_count", free_count, 1, i32),
+                           ("free_count_out", free_count_out, 1, i32),
+                           ("kv_lens", kv_lens, B, i32), ("cu_tokens", cu_tokens, B + 1, i32),
+                           ("seq_ids", seq_ids, num_rows, i32),
+                           ("positions", positions, num_rows, i32),
+                           ("slot_rows", slot_rows, num_rows, torch.int64),
+                           ("free_pages", free_pages, free_pages.shape[0], i32)):
+        if t.dtype != dt or t.shape != (n,) or not t.is_contiguous():
+            raise HelmError(f"build_step_tables: {name} must be contiguous {dt} [{n}]")
+    if (page_table.dtype != i32 or page_table.dim() != 2 or page_table.shape[0] != B
+            or page_table.stride(1) != 1):
+        raise HelmError("build_step_tables: page_table must be int32 [B, max_pages] with "
+                        "contiguous rows")
+    with _on_device(dev):
+        rc = lib().helm_build_step_tables(
+            past_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+            page_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+            free_count_out.data_ptr(), kv_lens.data_ptr(), cu_tokens.data_ptr(),
+            seq_ids.data_ptr(), positions.data_ptr(), slot_rows.data_ptr(), B, page_size, num_rows,
+            _stream_handle(dev, stream))
+    _check(rc, "helm_build_step_tables")
+    return kv_lens, cu_tokens, seq_ids, positions, slot_rows
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
+                  temperature: Optional[torch.Tensor] = None,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  logprobs: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """One token per row of logits [B, V] (bf16, fp16 or fp32, unit inner stride)
+    from the given uniforms fp32 [B] in [0, 1).  temperature, top_p, min_p fp32
+    [B] and top_k int32 [B], each optional; a temperature of 0 takes the largest
+    logit.  Returns ids int64 [B] (-1: nothing to draw from); logprobs fp32 [B]
+    gets the tokens' log softmax(l / T).  include/helm_b200.h has the definition.
+    """
+    dev = logits.device
+    _on("sample_tokens", dev, uniforms=uniforms, temperature=temperature, top_k=top_k,
+        top_p=top_p, min_p=min_p, out=out, logprobs=logprobs)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise HelmError("sample_tokens: logits must be [B, V] with a unit inner stride")
+    B, V = logits.shape
+    for name, t, dt in (("uniforms", uniforms, torch.float32),
+                        ("temperature", temperature, torch.float32),
+                        ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32), ("out", out, torch.int64),
+                        ("logprobs", logprobs, torch.float32)):
+        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
+            raise HelmError(f"sample_tokens: {name} must be contiguous {dt} [{B}]")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=dev)
+    with _on_device(dev):
+        rc = lib().helm_sample_tokens(
+            logits.data_ptr(), logits.stride(0), helm_dtype(logits.dtype), uniforms.data_ptr(),
+            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(),
+            _ptr(logprobs), B, V, _stream_handle(dev, stream))
+    _check(rc, "helm_sample_tokens")
+    return out

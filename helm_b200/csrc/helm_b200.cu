@@ -14,6 +14,10 @@
 #include "paged_prefill_tc.cu"
 #include "peer_exchange.cu"
 #include "decode_gemv.cu"
+#include "step_tables.cu"
+#include "kv_fp4.cu"
+#include "paged_attention_fp4.cu"
+#include "sample_tokens.cu"
 
 namespace helm {
 

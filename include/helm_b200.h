@@ -37,6 +37,8 @@ extern "C" {
 #define HELM_DEV_TIMEOUT 1u   /* a bounded wait inside a kernel gave up      */
 #define HELM_DEV_BAD_PAGE 2u  /* a page-table entry or page count was out of */
                               /* range; the access was skipped / clamped     */
+#define HELM_DEV_NO_PAGES 4u  /* helm_build_step_tables refused a request: its */
+                              /* page-table row or the free pages ran out      */
 
 /* ---- data types ------------------------------------------------------------ */
 #define HELM_DTYPE_FP32 0
@@ -364,6 +366,137 @@ int helm_decode_gemv_allreduce(void* const* bufs, int rank, int world, const voi
                                int64_t y_stride, int batch, int dtype, uint64_t timeout_ns,
                                void* stream);
 int64_t helm_decode_gemv_allreduce_bytes(int64_t n, int batch, int world);
+
+/*
+ * ---- 4-bit pages ----------------------------------------------------------
+ * A pool of 4-bit pages is uint8 [pool_pages, Hkv, page_size/16, 18*D]: per KV
+ * head one tile per 16 tokens, 4.5 bits a value.  16 consecutive values of a
+ * head row share an e4m3 scale s = e4m3(max|x| / 6) (nearest, saturating at
+ * 448); a value is the nearest e2m1 number (0 .5 1 1.5 2 3 4 6, ties to even)
+ * to x / s, times s.  A block that holds a NaN reads back as NaN; infinities
+ * saturate.  k_scale and v_scale are scales of the whole cache, powers of two
+ * between 2^-60 and 2^60 (1 where blocks' maxima lie between 2^-4 and 2688):
+ * rows are divided by them on the way in and multiplied on the way out.
+ * A tile's bytes: K codes [0, 8D), V codes [8D, 16D), K scales [16D, 17D), V
+ * scales [17D, 18D), ordered for the decode kernel (helm_b200/csrc/fp4.cuh).
+ * page_size is a multiple of 16; head_dim is 64, 128 or 256; the pool is
+ * 16-byte aligned.  helm_copy_pages moves such pages like any others
+ * (page_bytes from helm_fp4_page_bytes, -1 for an unsupported shape).  HELM
+ * keeps its cache in the model's dtype: no counterpart there.
+ */
+int64_t helm_fp4_page_bytes(int num_kv_heads, int page_size, int head_dim);
+
+/*
+ * helm_kv_append for 4-bit pages: optional RMSNorm of q and k, optional rotary
+ * embedding (rotate_half convention), K and V rows quantised into pool row
+ * slot_rows[token] = slot*page_size + row_in_page (negative: skipped).  The
+ * rows of one call are distinct.  All of it is computed in fp32: q_out rounds
+ * once to `dtype`, K and V once to 4 bits.  Arguments as helm_kv_append, with
+ * 16-byte aligned pointers and strides that are multiples of 8 elements; q and
+ * q_out are given together or not at all.
+ */
+int helm_kv_append_fp4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                       int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                       int64_t v_stride_h, const void* q_norm_w, const void* k_norm_w, float eps,
+                       const void* cos, const void* sin, int64_t rope_stride_t, void* q_out,
+                       int64_t q_out_stride_t, int64_t q_out_stride_h, void* kv_pool,
+                       int64_t pool_pages, const int64_t* slot_rows, int num_tokens,
+                       int num_q_heads, int num_kv_heads, int head_dim, int page_size, int dtype,
+                       float k_scale, float v_scale, void* stream);
+
+/*
+ * The rows slot_rows[0 .. num_tokens) of a 4-bit pool as the values they stand
+ * for: k_out, v_out [num_tokens, Hkv, D] in dtype (exact in bf16 and fp16 for
+ * cache scales of 1), with token and head strides (multiples of 8 elements,
+ * 16-byte aligned).  A negative row gives zeros.  The 4-bit counterpart of
+ * helm_gather_kv, by rows: of helm_build_step_tables, or of a chunk that a
+ * dense attention reads.
+ */
+int helm_gather_kv_rows_fp4(const void* kv_pool, int64_t pool_pages, const int64_t* slot_rows,
+                            void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h,
+                            void* v_out, int64_t v_out_stride_t, int64_t v_out_stride_h,
+                            int num_tokens, int num_kv_heads, int head_dim, int page_size,
+                            int dtype, float k_scale, float v_scale, void* stream);
+
+/*
+ * helm_paged_decode_attention over 4-bit pages: same computation, arguments and
+ * overlap setting, without ragged page lists (page i of sequence b holds
+ * tokens i*page_size ..), O in the query dtype.  A key whose mask value is -inf
+ * contributes nothing, whatever its page holds, NaN included; a row that sees
+ * no key gets O = 0, LSE = -inf.  q: 4-byte aligned, even strides.
+ *  workspace  >= helm_paged_decode_fp4_workspace_bytes(...) bytes, 256-byte
+ *             aligned, any contents; calls that overlap on the GPU need one each
+ */
+int64_t helm_paged_decode_fp4_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                              int head_dim);
+int helm_paged_decode_attention_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                    const void* kv_pool, int64_t pool_pages,
+                                    const int32_t* page_table, int64_t pt_stride_b, int max_pages,
+                                    const int32_t* kv_lens, const void* mask, int mask_dtype,
+                                    int64_t mask_stride_b, void* out, int64_t out_stride_b,
+                                    int64_t out_stride_h, float* lse, void* workspace,
+                                    int64_t workspace_bytes, int batch, int num_q_heads,
+                                    int num_kv_heads, int head_dim, int page_size, int dtype,
+                                    float scale, float softcap, float k_scale, float v_scale,
+                                    int max_kv_len_hint, void* stream);
+
+/*
+ * Page tables, slot rows and positions of one step of a continuous batch, from
+ * the requests' lengths, on the device.
+ *  past_lens    int32 [B] tokens cached (negative counts as 0)
+ *  new_lens     int32 [B] tokens that the step appends (0: idle); negative: the
+ *               request leaves and gives its pages back
+ *  page_table   int32 [B, max_pages] (row stride pt_stride_b): entries of the
+ *               ceil(past/page_size) pages held are read; those of the pages
+ *               that the new tokens need are written; others stay as they are
+ *  free_pages   int32 [free_capacity]: stack of free pages, *free_count of them.
+ *               Pages given back are pushed request by request, then the fresh
+ *               pages are popped from the top, request by request.
+ *  free_count_out  the count afterwards (may be free_count itself)
+ *  kv_lens      int32 [B] out: past + new (0 for a request that left); may be
+ *               past_lens
+ *  cu_tokens    int32 [B + 1] out: tokens of the step before each request
+ *  seq_ids, positions (optional), slot_rows [num_rows] out: request, position
+ *               and pool row of token t; behind the last token -1, 0 and -1
+ * A request is refused when its row of the table is too short or the pages
+ * wanted up to and including it (those of requests refused for want of pages
+ * included) exceed the free ones: its length and pages stay, its tokens' rows
+ * are -1, and HELM_DEV_NO_PAGES is recorded.  free_count_out apart, a repeated
+ * call with the same inputs gives the same outputs.  B <= 8192;
+ * B * max_pages, max_pages * page_size and the sum of new_lens below 2^31.
+ *
+ * Replaces the host bookkeeping of KVAllocator.allocate / free
+ * (helm/runtime/kv_allocator.py:36-93) where a step runs without the host.
+ */
+int helm_build_step_tables(const int32_t* past_lens, const int32_t* new_lens, int32_t* page_table,
+                           int64_t pt_stride_b, int max_pages, int32_t* free_pages,
+                           int free_capacity, const int32_t* free_count, int32_t* free_count_out,
+                           int32_t* kv_lens, int32_t* cu_tokens, int32_t* seq_ids,
+                           int32_t* positions, int64_t* slot_rows, int batch, int page_size,
+                           int num_rows, void* stream);
+
+/*
+ * Samples one token per row of logits [batch, vocab] (row stride row_stride,
+ * unit inner stride; bf16, fp16 or fp32; vocab <= 262144).  Candidates are
+ * ordered by (logit descending, index ascending), w_i = exp((l_i - l_max)/T):
+ *  temperature [batch] fp32 (NULL: 1); T <= 0 or NaN: the first candidate
+ *  top_k       [batch] int32 (NULL, <= 0 or >= vocab: all): the first k
+ *  top_p       [batch] fp32 (NULL or >= 1: all): of those, the shortest prefix
+ *              whose weights reach top_p of their sum (one candidate at least)
+ *  min_p       [batch] fp32 (NULL or <= 0: all): w_i >= min_p
+ *  uniforms    [batch] fp32 in [0, 1): the token is the smallest index whose
+ *              running sum of kept weights, in index order, exceeds u * their sum
+ *  ids         [batch] int64 out; -1 for a row without a candidate above -inf
+ *  logprobs    optional fp32 [batch] out: log softmax(l / T) of the token over
+ *              the whole row (T = 1 where T <= 0), -inf where ids is -1
+ * NaN logits count as -inf.  The result does not depend on the launch: weights
+ * are summed as 64-bit integers.  The reference decodes greedily only
+ * (helm/runtime/pipeline_runtime.py:300-338).
+ */
+int helm_sample_tokens(const void* logits, int64_t row_stride, int dtype, const float* uniforms,
+                       const float* temperature, const int32_t* top_k, const float* top_p,
+                       const float* min_p, int64_t* ids, float* logprobs, int batch, int vocab,
+                       void* stream);
 
 #ifdef __cplusplus
 }
