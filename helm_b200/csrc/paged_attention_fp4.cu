@@ -20,17 +20,21 @@
 //   * V fragments pair two tokens of one dim.  Nibbles of two token words are
 //     interleaved before widening (four logic ops per 16 values).
 //   * The running maximum moves only when a score exceeds it by 8 in log2
-//     units (then P <= 2^8, far inside fp16), so a tile normally costs one
+//     units (then P <= 2^8, far inside fp16), so a unit normally costs one
 //     vote instead of a max reduction and a rescale of O.
-//   * q is scaled per head by a power of two into fp16's range; P is rounded
-//     to fp16 (2^-12 relative); the sum l and all state stay fp32.
+//   * Work goes by UNITS of two tiles (32 tokens): their chains of LDS, cvt,
+//     mma and exp2 are independent, and waits, votes and bookkeeping are paid
+//     once for both.
+// q is scaled per head by a power of two into fp16's range.  P is rounded to
+// fp16 (half a step: 2^-11) where O is bf16 (2^-8); where O is fp16 itself it
+// is carried as the sum of two fp16 numbers.  The sum l and all state are fp32.
 //
-// Work split and merge follow paged_attention.cu: all tiles of all (sequence,
-// KV head) pairs in one flattened order, cut into equal contiguous ranges, one
-// per warp; a warp's ring of bulk copies is its own (its next copy is issued
-// by the warp itself once the stage is read), so no producer warp and no empty
-// barriers are needed.  States of warps that end in the same pair are combined
-// in the CTA; pairs split across CTAs by a programmatic-dependent merge kernel.
+// All units of all (sequence, KV head) pairs lie in one flattened order, cut into
+// equal contiguous ranges, one per warp (paged_attention.cu's split).  A warp's
+// ring of bulk copies is its own (its next copy is issued by the warp itself
+// once the stage is read), so no producer warp and no empty barriers are
+// needed.  Pairs split across warps are merged by a programmatic-dependent
+// kernel.
 #include "common.cuh"
 #include "fp4.cuh"
 
@@ -54,37 +58,39 @@ struct DecodeFp4Args {
   float* lse;
   float* part_o;   // warp partials [num_workers + pairs][G][D]
   float* part_ml;  // warp partials [num_workers + pairs][G][2]
-  float* cta_o;    // CTA partials [grid + pairs][G][D]
-  float* cta_ml;
   int batch, hq, hkv, group, page_size, tiles_per_page;
+  uint32_t tpp_magic;  // x / tiles_per_page = (x * tpp_magic) >> 32 for x < 2^31 / 16, 0: shift
+  int tpp_shift;
+  int warps;         // workers of a CTA
   int num_workers;
-  int plain;         // no mask, no softcap, scale > 0: scores stay unscaled
+  int early;         // decode overlap: the lengths and tables may be read before the wait
   float score_scale; // softmax scale x K cache scale
   float softcap;
   float v_scale;
-  // A state's maximum m is in log2 units when `plain`, in natural units of the
-  // score otherwise (a mask of the type's lowest value must not overflow):
+  // A state's maximum m is in log2 units in the plain form (no mask, no softcap,
+  // scale > 0), in natural units of the score otherwise (a mask of the type's
+  // lowest value must not overflow):
   float unit_log2;   // exp2 factor of a difference of maxima: 1 or log2(e)
   float unit_ln;     // natural units of m: ln 2 or 1
 };
 
 constexpr float kLowest = -3.402823466e38f;
+constexpr int kUnitTokens = 2 * kFp4TileTokens;
+constexpr int kFp4MaxWarps = 16;  // of a CTA (sizes the workspace)
 
-// Shape of a CTA: consumer warps and ring stages per warp.
+// Shape of a CTA: warps (= workers) and ring stages (of one unit) per warp.
 template <int D, int NT>
 struct Fp4Shape {
   static constexpr int NCW = (D <= 128 && NT == 1) ? 16 : 8;
-  static constexpr int NS = D == 64 ? 8 : (D == 128 && NT == 2 ? 8 : 5);
+  static constexpr int NS = D == 64 ? 4 : (NCW == 16 ? 2 : (D == 128 ? 4 : 2));
   static constexpr int kThreads = NCW * 32;
   static constexpr int kTile = Fp4Tile<D>::kBytes;
-  static constexpr int kHeads = 8 * NT;
-  static constexpr int kRec = 2 * kHeads + kHeads * D;  // floats of a warp's end state
-  static constexpr int kRing = NCW * NS * kTile;
-  static constexpr int kState = NCW * kRec * 4;
-  static constexpr int kData = ((kRing > kState ? kRing : kState) + 127) / 128 * 128;
+  static constexpr int kUnit = 2 * kTile;
+  static constexpr int kData = NCW * NS * kUnit;
   static constexpr size_t smem_bytes(int batch) {
-    return 128 + kData + NCW * NS * sizeof(uint64_t) + (batch + 1) * sizeof(int);
+    return 128 + kData + NCW * NS * sizeof(uint64_t) + (2 * batch + 1) * sizeof(int);
   }
+  static_assert(NCW <= kFp4MaxWarps, "");
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -126,22 +132,37 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
 __device__ __forceinline__ uint32_t bcast_lo(uint32_t h2) { return __byte_perm(h2, h2, 0x1010); }
 __device__ __forceinline__ uint32_t bcast_hi(uint32_t h2) { return __byte_perm(h2, h2, 0x3232); }
 
-__device__ __forceinline__ int fp4_tiles_of_seq(const DecodeFp4Args& a, int b) {
-  const int len = a.kv_lens[b];
-  if (len <= 0) return 0;
-  if (static_cast<int64_t>(len) > static_cast<int64_t>(a.max_pages) * a.page_size) {
-    report_status(HELM_DEV_BAD_PAGE);
-    return a.max_pages * a.tiles_per_page;
-  }
-  return div_up(len, kFp4TileTokens);
+// d = a . b (no accumulator to clear first)
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32"
+      " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-__device__ void fp4_build_prefix(const DecodeFp4Args& a, int* s_cum, int lane) {
+// Tokens of sequence b (a length beyond its row of the table is cut and reported).
+__device__ __forceinline__ int fp4_len(const DecodeFp4Args& a, int b) {
+  const int len = a.kv_lens[b];
+  const int64_t most = static_cast<int64_t>(a.max_pages) * a.page_size;
+  if (len > most) {
+    report_status(HELM_DEV_BAD_PAGE);
+    return static_cast<int>(most);
+  }
+  return max(len, 0);
+}
+
+// s_cum[b]: units of one KV head before sequence b, s_len[b]: its tokens (one
+// warp fills both).
+__device__ void fp4_build_prefix(const DecodeFp4Args& a, int* s_cum, int* s_len, int lane) {
   int carry = 0;
   if (lane == 0) s_cum[0] = 0;
   for (int base = 0; base < a.batch; base += 32) {
     const int b = base + lane;
-    int v = b < a.batch ? fp4_tiles_of_seq(a, b) : 0;
+    const int len = b < a.batch ? fp4_len(a, b) : 0;
+    if (s_len != nullptr && b < a.batch) s_len[b] = len;
+    int v = div_up(len, kUnitTokens);
     for (int off = 1; off < 32; off <<= 1) {
       const int n = __shfl_up_sync(0xffffffffu, v, off);
       if (lane >= off) v += n;
@@ -151,7 +172,6 @@ __device__ void fp4_build_prefix(const DecodeFp4Args& a, int* s_cum, int lane) {
   }
 }
 
-// Mask value of a token (0 without a mask).
 __device__ __forceinline__ float fp4_mask(const DecodeFp4Args& a, int b, int tok) {
   const int64_t off = static_cast<int64_t>(b) * a.mask_sb + tok;
   if (a.mask_dtype == HELM_DTYPE_FP32) return static_cast<const float*>(a.mask)[off];
@@ -170,38 +190,89 @@ __device__ __forceinline__ float fp4_lse(const DecodeFp4Args& a, float m, float 
   return l > 0.f ? m * a.unit_ln + logf(l) : (l == l ? -INFINITY : l);
 }
 
-// Where a pair's tiles lie in the flattened order (as PairSpan there).
+// O of a state is kept in the order in which lanes hold it: place i is this dim.
+template <int D>
+__device__ __forceinline__ int fp4_state_dim(int i) {
+  return (D / 8) * ((i >> 1) & 7) + 2 * (i >> 4) + (i & 1);
+}
+
+// x / y for x < 2^30 and a quotient below 2^20: the float product is at most one
+// off.  The kernel divides a handful of times per warp, at its start and end,
+// where nothing else runs: a general division there is microseconds in all.
+__device__ __forceinline__ int fp4_div(int x, int y) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
+  const int r = x - q * y;
+  q += r >= y ? 1 : 0;
+  q -= r < 0 ? 1 : 0;
+  return q;
+}
+
+// locate() of the flattened unit order with that division.
+__device__ __forceinline__ TilePos fp4_locate(const int* s_cum, int batch, int hkv, int x) {
+  int lo = 0, hi = batch - 1;
+  while (lo < hi) {  // largest b with s_cum[b] * hkv <= x
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_cum[mid] * hkv <= x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int tb = s_cum[lo + 1] - s_cum[lo];
+  const int r = x - s_cum[lo] * hkv;
+  TilePos p;
+  p.b = lo;
+  p.h = fp4_div(r, tb);
+  p.t = r - p.h * tb;
+  return p;
+}
+
+// The workers vf .. vl whose ranges hold units of KV head h of sequence b.
 struct Fp4Span {
-  int tiles, vf, vl;
-  bool last_continues;
+  int vf, vl;
 };
 
-__device__ __forceinline__ Fp4Span fp4_span(const int* s_cum, int hkv, int W, int total, int b,
+__device__ __forceinline__ Fp4Span fp4_span(const DecodeFp4Args& a, const int* s_cum, int W, int b,
                                             int h) {
+  const int units = s_cum[b + 1] - s_cum[b], st = s_cum[b] * a.hkv + h * units;
   Fp4Span ps;
-  ps.tiles = s_cum[b + 1] - s_cum[b];
-  ps.vf = ps.vl = 0;
-  ps.last_continues = false;
-  if (ps.tiles > 0) {
-    const int st = s_cum[b] * hkv + h * ps.tiles, en = st + ps.tiles;
-    ps.vf = st / W;
-    ps.vl = (en - 1) / W;
-    ps.last_continues = static_cast<int64_t>(ps.vl + 1) * W > en && en < total;
-  }
+  ps.vf = fp4_div(st, W);
+  ps.vl = fp4_div(st + units - 1, W);
   return ps;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kPlain>
 struct Fp4Worker {
   static constexpr int KS = D / 16;
+  static constexpr bool kSplitP = std::is_same<T, __half>::value;
   using L = Fp4Tile<D>;
-  float m[NT][2];       // scores' units: unscaled dot products (plain) or natural
+  float m[NT][2];       // running maximum (units: see DecodeFp4Args), it may lag by 2^8
   float l[NT][2];
   float o[NT][KS][4];
   uint32_t qf[NT][KS][2];
-  float xs[NT][2];      // natural score = dot * xs
-  float cx[NT][2];      // exp2 factor of a difference of scores
-  int cur_b = -1, cur_h = -1, cur_len = 0;
+  float cx[NT][2];      // plain: dot product to log2 units; else to the natural score
+  int cur_b = -1, cur_h = -1;
+  // byte offsets in a tile of what this lane reads (kept: they cost more to redo)
+  uint32_t kA, kB, kS, v0, v1, v2, v3, vS;
+
+  // A lane's K rows: row i of S^T (i < 8: r, else r + 8) is token 4 (r >> 1) +
+  // (r & 1) [+ 2]; its V tokens: 4c .. 4c + 3.
+  __device__ __forceinline__ void lane_offsets(int lane) {
+    const int r = lane >> 2, c = lane & 3;
+    const int tA = 4 * (r >> 1) + (r & 1);
+    const int at = D == 64 ? c * 8 : (D == 128 ? c * 16 : (c ^ (4 * (r & 1))) * 16);
+    kA = L::row_of(tA) * L::kRow + at;
+    kB = L::row_of(tA + 2) * L::kRow + at;
+    kS = L::kKScale + lane * (D / 32);
+    const int chunk = L::kV + (r ^ L::v_turn(4 * c)) * (D / 16);
+    v0 = chunk + L::row_of(4 * c) * L::kRow;
+    v1 = chunk + L::row_of(4 * c + 1) * L::kRow;
+    v2 = chunk + L::row_of(4 * c + 2) * L::kRow;
+    v3 = chunk + L::row_of(4 * c + 3) * L::kRow;
+    vS = L::kVScale + (D == 64 ? r >> 1 : (D == 128 ? r : 2 * r)) * 16 + 4 * c;
+    // opaque to the compiler, which would rather compute them again at every use
+    asm volatile("" : "+r"(kA), "+r"(kB), "+r"(kS), "+r"(vS));
+    asm volatile("" : "+r"(v0), "+r"(v1), "+r"(v2), "+r"(v3));
+  }
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -272,14 +343,9 @@ struct Fp4Worker {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float bk = __shfl_sync(0xffffffffu, back, (2 * c + j) * 4);
-        xs[nt][j] = a.score_scale * bk;
-        cx[nt][j] = a.plain ? xs[nt][j] * kLog2e : kLog2e;
+        cx[nt][j] = a.score_scale * bk * (kPlain ? kLog2e : 1.f);
       }
     }
-  }
-
-  __device__ __forceinline__ float m_unit(const DecodeFp4Args& a, int nt, int j) const {
-    return a.plain ? fmaxf(m[nt][j] * cx[nt][j], kLowest) : m[nt][j];
   }
 
   // Ends the current pair: the final output when this warp covered the whole
@@ -292,7 +358,6 @@ struct Fp4Worker {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float lt = warp_sum_xor(l[nt][j], 4, 16);
-        const float mu = m_unit(a, nt, j);
         const int hg = nt * 8 + 2 * c + j;
         if (hg >= a.group) continue;
         if (alone) {
@@ -305,171 +370,206 @@ struct Fp4Worker {
             po[2 * mt + 1] = from_float<T>(o[nt][mt][2 + j] * inv);
           }
           if (r == 0 && a.lse != nullptr)
-            a.lse[static_cast<int64_t>(cur_b) * a.hq + qh] = fp4_lse(a, mu, lt);
+            a.lse[static_cast<int64_t>(cur_b) * a.hq + qh] = fp4_lse(a, m[nt][j], lt);
         } else {
           const int64_t slot = static_cast<int64_t>(v + p) * a.group + hg;
-          float* po = a.part_o + slot * D + r * (D / 8);
+          float* po = a.part_o + slot * D + 2 * r;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
-            *reinterpret_cast<float2*>(po + 2 * mt) = make_float2(o[nt][mt][j], o[nt][mt][2 + j]);
-          if (r == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(mu, lt);
+            *reinterpret_cast<float2*>(po + 16 * mt) = make_float2(o[nt][mt][j], o[nt][mt][2 + j]);
+          if (r == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m[nt][j], lt);
         }
       }
     }
   }
 
-  // End state into a shared-memory record m[kHeads] | l[kHeads] | O[kHeads][D].
-  __device__ __forceinline__ void save(const DecodeFp4Args& a, float* rec, int lane) {
-    constexpr int kHeads = 8 * NT;
-    const int r = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float lt = warp_sum_xor(l[nt][j], 4, 16);
-        const float mu = m_unit(a, nt, j);
-        const int hg = nt * 8 + 2 * c + j;
-        if (hg >= a.group) continue;
-        float* po = rec + 2 * kHeads + hg * D + r * (D / 8);
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt)
-          *reinterpret_cast<float2*>(po + 2 * mt) = make_float2(o[nt][mt][j], o[nt][mt][2 + j]);
-        if (r == 0) {
-          rec[hg] = mu;
-          rec[kHeads + hg] = lt;
-        }
-      }
+  // S^T = K . Q^T of the tile at shared address `base`.
+  __device__ __forceinline__ void scores(uint32_t base, float (&s)[NT][4]) {
+    constexpr int kHalves = D == 256 ? 2 : 1;  // 32-dim chunks of a lane
+    constexpr int kWords = D == 64 ? 2 : 4;    // code words per chunk
+    float s2[NT][4];
+    uint32_t scA[2], scB[2];  // f16x2 scale pairs per chunk
+    if (D == 64) {
+      const uint32_t two = e4m3x2_to_half2(lds_u16(base + kS));
+      scA[0] = bcast_lo(two);
+      scB[0] = bcast_hi(two);
+    } else if (D == 128) {
+      uint32_t w[1];
+      lds_words<1>(base + kS, w);
+      scA[0] = e4m3x2_to_half2(w[0]);
+      scB[0] = e4m3x2_to_half2(w[0] >> 16);
+    } else {
+      uint32_t w[2];
+      lds_words<2>(base + kS, w);
+      scA[0] = e4m3x2_to_half2(w[0]);
+      scA[1] = e4m3x2_to_half2(w[0] >> 16);
+      scB[0] = e4m3x2_to_half2(w[1]);
+      scB[1] = e4m3x2_to_half2(w[1] >> 16);
     }
-  }
-
-  // One tile at shared address `base`; its first token is tok0, the first
-  // `valid` of its 16 tokens exist.
-  __device__ __forceinline__ void tile(const DecodeFp4Args& a, uint32_t base, int valid, int tok0,
-                                       int lane) {
-    const int r = lane >> 2, c = lane & 3;
-    // ---- S^T = K . Q^T.  Row i of the product (i < 8: r, else r + 8) is token
-    // 4 (r >> 1) + (r & 1) [+ 2]: then the transposed P has the token order in
-    // which a lane reads V (tokens 4c .. 4c + 3).
-    const int tA = 4 * (r >> 1) + (r & 1), tB = tA + 2;
-    const int turn = ((r & 2)) | (r >> 2);  // row_of(t) ^ t of both tokens
-    float s[NT][4];
-    {
-      float s2[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int hf = 0; hf < kHalves; ++hf) {
+      uint32_t wa[kWords], wb[kWords];
+      // the second chunk of D = 256 is 64 bytes on, modulo the row's turn
+      lds_words<kWords>(base + (kA ^ (64 * hf)), wa);
+      lds_words<kWords>(base + (kB ^ (64 * hf)), wb);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
-      constexpr int kHalves = D == 256 ? 2 : 1;         // 32-dim chunks of a lane
-      constexpr int kWords = D == 64 ? 2 : 4;           // code words per chunk
-      uint32_t scA[2], scB[2];                          // f16x2 scale pairs per chunk
-      if (D == 64) {
-        const uint32_t two = e4m3x2_to_half2(lds_u16(base + L::kKScale + lane * 2));
-        scA[0] = bcast_lo(two);
-        scB[0] = bcast_hi(two);
-      } else if (D == 128) {
-        uint32_t w[1];
-        lds_words<1>(base + L::kKScale + lane * 4, w);
-        scA[0] = e4m3x2_to_half2(w[0]);
-        scB[0] = e4m3x2_to_half2(w[0] >> 16);
-      } else {
-        uint32_t w[2];
-        lds_words<2>(base + L::kKScale + lane * 8, w);
-        scA[0] = e4m3x2_to_half2(w[0]);
-        scA[1] = e4m3x2_to_half2(w[0] >> 16);
-        scB[0] = e4m3x2_to_half2(w[1]);
-        scB[1] = e4m3x2_to_half2(w[1] >> 16);
-      }
+      for (int w = 0; w < kWords; ++w) {
+        uint32_t ha[4], hb[4];
+        fp4x8_to_half(wa[w], ha);
+        fp4x8_to_half(wb[w], hb);
+        const uint32_t sa = D == 64 ? scA[0] : (w < 2 ? bcast_lo(scA[hf]) : bcast_hi(scA[hf]));
+        const uint32_t sb = D == 64 ? scB[0] : (w < 2 ? bcast_lo(scB[hf]) : bcast_hi(scB[hf]));
 #pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf) {
-        uint32_t wa[kWords], wb[kWords];
-        const uint32_t at = D == 64 ? c * 8 : (D == 128 ? c * 16 : ((c + 4 * hf) ^ (4 * (r & 1))) * 16);
-        lds_words<kWords>(base + (tA ^ turn) * L::kRow + at, wa);
-        lds_words<kWords>(base + (tB ^ turn) * L::kRow + at, wb);
+        for (int e = 0; e < 2; ++e) {  // two k-steps per code word
+          const int kk = hf * 8 + 2 * w + e;
+          uint32_t af[4] = {hmul2(ha[2 * e], sa), hmul2(hb[2 * e], sb), hmul2(ha[2 * e + 1], sa),
+                            hmul2(hb[2 * e + 1], sb)};
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-          uint32_t ha[4], hb[4];
-          fp4x8_to_half(wa[w], ha);
-          fp4x8_to_half(wb[w], hb);
-          const uint32_t sa = D == 64 ? scA[0] : (w < 2 ? bcast_lo(scA[hf]) : bcast_hi(scA[hf]));
-          const uint32_t sb = D == 64 ? scB[0] : (w < 2 ? bcast_lo(scB[hf]) : bcast_hi(scB[hf]));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {  // two k-steps per code word
-            const int kk = hf * 8 + 2 * w + e;
-            uint32_t af[4] = {hmul2(ha[2 * e], sa), hmul2(hb[2 * e], sb), hmul2(ha[2 * e + 1], sa),
-                              hmul2(hb[2 * e + 1], sb)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            if (kk < 2)
+              mma_f16_zero(e ? s2[nt] : s[nt], af, qf[nt][kk][0], qf[nt][kk][1]);
+            else
               MmaOp<__half>::run(e ? s2[nt] : s[nt], af, qf[nt][kk][0], qf[nt][kk][1]);
           }
         }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
     }
-    // ---- scores -> probabilities ---------------------------------------------
-    uint32_t keep01 = 0xffffffffu, keep23 = 0xffffffffu;  // V tokens 4c..4c+3 that count
-    if (!a.plain) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = s[nt][e] * xs[nt][e & 1];
-          if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-          s[nt][e] = x;
-        }
-    }
-    bool seeA = true, seeB = true;
-    if (valid < kFp4TileTokens) {
-      seeA = tA < valid;
-      seeB = tB < valid;
-    }
-    if (a.mask != nullptr) {
-      const float mA = seeA ? fp4_mask(a, cur_b, tok0 + tA) : -INFINITY;
-      const float mB = seeB ? fp4_mask(a, cur_b, tok0 + tB) : -INFINITY;
-      seeA = mA != -INFINITY;
-      seeB = mB != -INFINITY;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          s[nt][j] += mA;
-          s[nt][2 + j] += mB;
-        }
-    }
-    if (__any_sync(0xffffffffu, !(seeA && seeB))) {
-      // an excluded key contributes nothing, whatever its page holds: its score
-      // is -inf and its V scales are cleared (codes are finite, scales may be NaN)
-      const unsigned eA = __ballot_sync(0xffffffffu, seeA), eB = __ballot_sync(0xffffffffu, seeB);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (!seeA) s[nt][j] = -INFINITY;
-          if (!seeB) s[nt][2 + j] = -INFINITY;
-        }
-      // token 4c + i is row r' = 2c + (i & 1) of A (i < 2) or B: lane 4 r'
-      keep01 = ((eA >> (8 * c)) & 1 ? 0x0000ffffu : 0u) | ((eA >> (8 * c + 4)) & 1 ? 0xffff0000u : 0u);
-      keep23 = ((eB >> (8 * c)) & 1 ? 0x0000ffffu : 0u) | ((eB >> (8 * c + 4)) & 1 ? 0xffff0000u : 0u);
-    }
-    float t[NT][4];
-    bool high = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        t[nt][e] = (s[nt][e] - m[nt][e & 1]) * cx[nt][e & 1];
-        high |= t[nt][e] > 8.f;
+      for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+  }
+
+  // O^T += V^T . P^T of the tile at `base`; pb: P fragments (and their low
+  // halves), keep: lanes' tokens 4c .. 4c+3 that count, as f16x2 masks.  Row r
+  // (r + 8) of m-tile mt is dim D/8 r + 2 mt (+ 1).
+  __device__ __forceinline__ void values(uint32_t base, const uint32_t (&pb)[NT][2],
+                                         const uint32_t (&pl)[NT][2], uint32_t keep01,
+                                         uint32_t keep23) {
+    constexpr int kWords = D / 64 < 1 ? 1 : D / 64;  // code words of a lane per token
+    uint32_t w[4][kWords];
+    lds_words<kWords>(base + v0, w[0]);
+    lds_words<kWords>(base + v1, w[1]);
+    lds_words<kWords>(base + v2, w[2]);
+    lds_words<kWords>(base + v3, w[3]);
+    uint32_t sc01[2], sc23[2];
+    constexpr int kGroups = D == 256 ? 2 : 1;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      uint32_t sw[1];
+      lds_words<1>(base + vS + g * 16, sw);
+      sc01[g] = e4m3x2_to_half2(sw[0]) & keep01;
+      sc23[g] = e4m3x2_to_half2(sw[0] >> 16) & keep23;
+    }
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) {
+      constexpr uint32_t kLo = 0x0f0f0f0fu, kHi = 0xf0f0f0f0u;
+      uint32_t e01[4], d01[4], e23[4], d23[4];
+      fp4x8_to_half((w[0][q] & kLo) | ((w[1][q] << 4) & kHi), e01);  // even dims of tokens 0, 1
+      fp4x8_to_half(((w[0][q] >> 4) & kLo) | (w[1][q] & kHi), d01);  // odd dims
+      fp4x8_to_half((w[2][q] & kLo) | ((w[3][q] << 4) & kHi), e23);
+      fp4x8_to_half(((w[2][q] >> 4) & kLo) | (w[3][q] & kHi), d23);
+      const int g = D == 256 ? q >> 1 : 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t af[4] = {hmul2(e01[b], sc01[g]), hmul2(d01[b], sc01[g]), hmul2(e23[b], sc23[g]),
+                          hmul2(d23[b], sc23[g])};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          MmaOp<__half>::run(o[nt][4 * q + b], af, pb[nt][0], pb[nt][1]);
+          if (kSplitP) MmaOp<__half>::run(o[nt][4 * q + b], af, pl[nt][0], pl[nt][1]);
+        }
       }
-    if (__any_sync(0xffffffffu, high)) {
+    }
+  }
+
+  // One unit at shared address `base`.  kFull: all of its 32 tokens exist and
+  // no mask is given; else its first token is tok0 and `valid` (1 .. 32) exist.
+  template <bool kFull>
+  __device__ __forceinline__ void unit(const DecodeFp4Args& a, uint32_t base, int valid, int tok0,
+                                       int lane) {
+    float s[2][NT][4];
+    scores(base, s[0]);
+    scores(base + L::kBytes, s[1]);
+    uint32_t keep01[2] = {0xffffffffu, 0xffffffffu}, keep23[2] = {0xffffffffu, 0xffffffffu};
+    if (!kPlain) {
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = s[ti][nt][e] * cx[nt][e & 1];
+            if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+            s[ti][nt][e] = x;
+          }
+    }
+    if (!kFull) {
+      const int r = lane >> 2, c = lane & 3;
+      const int tA = 4 * (r >> 1) + (r & 1), tB = tA + 2;
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti) {
+        const int v = valid - ti * kFp4TileTokens;
+        bool seeA = tA < v, seeB = tB < v;
+        if (!kPlain && a.mask != nullptr) {
+          const int t0 = tok0 + ti * kFp4TileTokens;
+          const float mA = seeA ? fp4_mask(a, cur_b, t0 + tA) : -INFINITY;
+          const float mB = seeB ? fp4_mask(a, cur_b, t0 + tB) : -INFINITY;
+          seeA = mA != -INFINITY;
+          seeB = mB != -INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              s[ti][nt][j] += mA;
+              s[ti][nt][2 + j] += mB;
+            }
+        }
+        // an excluded key contributes nothing, whatever its page holds: its score
+        // is -inf and its V scales are cleared (codes are finite, scales may be NaN)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (!seeA) s[ti][nt][j] = -INFINITY;
+            if (!seeB) s[ti][nt][2 + j] = -INFINITY;
+          }
+        // token 4c + i is row r' = 2c + (i & 1) of A (i < 2) or B: lane 4 r'
+        const unsigned eA = __ballot_sync(0xffffffffu, seeA);
+        const unsigned eB = __ballot_sync(0xffffffffu, seeB);
+        keep01[ti] =
+            ((eA >> (8 * c)) & 1 ? 0x0000ffffu : 0u) | ((eA >> (8 * c + 4)) & 1 ? 0xffff0000u : 0u);
+        keep23[ti] =
+            ((eB >> (8 * c)) & 1 ? 0x0000ffffu : 0u) | ((eB >> (8 * c + 4)) & 1 ? 0xffff0000u : 0u);
+      }
+    }
+    // exponents against the running maximum; it moves when one exceeds 8
+    float t[2][NT][4];
+    auto exponents = [&]() {
+      float hi = -1.f;
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[ti][nt][e];
+            t[ti][nt][e] = kPlain ? fmaf(x, cx[nt][e & 1], -m[nt][e & 1])
+                                  : (x - m[nt][e & 1]) * kLog2e;
+            hi = fmaxf(hi, t[ti][nt][e]);
+          }
+      return hi;
+    };
+    if (__any_sync(0xffffffffu, exponents() > 8.f)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float mx = warp_max_xor(fmaxf(s[nt][j], s[nt][2 + j]), 4, 16);
+          float mx = fmaxf(fmaxf(s[0][nt][j], s[0][nt][2 + j]), fmaxf(s[1][nt][j], s[1][nt][2 + j]));
+          mx = warp_max_xor(mx, 4, 16);
+          if (kPlain) mx *= cx[nt][j];
           const float m_new = fmaxf(m[nt][j], mx);
-          const float alpha = exp2_fast((m[nt][j] - m_new) * cx[nt][j]);
+          const float alpha = exp2_fast((m[nt][j] - m_new) * (kPlain ? 1.f : kLog2e));
           m[nt][j] = m_new;
           l[nt][j] *= alpha;
 #pragma unroll
@@ -477,108 +577,54 @@ struct Fp4Worker {
             o[nt][mt][j] *= alpha;
             o[nt][mt][2 + j] *= alpha;
           }
-          t[nt][j] = (s[nt][j] - m_new) * cx[nt][j];
-          t[nt][2 + j] = (s[nt][2 + j] - m_new) * cx[nt][j];
         }
+      exponents();
     }
-    uint32_t pb0[NT], pb1[NT];
+    uint32_t pb[2][NT][2], pl[2][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
+    for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(t[nt][e]);
-      l[nt][0] += p[0] + p[2];
-      l[nt][1] += p[1] + p[3];
-      pb0[nt] = movmatrix_trans(MmaOp<__half>::pack(p[0], p[1]));
-      pb1[nt] = movmatrix_trans(MmaOp<__half>::pack(p[2], p[3]));
-    }
-    // ---- O^T += V^T . P^T: row r (r + 8) of m-tile mt is dim D/8 r + 2 mt (+ 1)
-    {
-      constexpr int kWords = D / 64 < 1 ? 1 : D / 64;  // code words of a lane per token
-      const int vturn = D == 128 ? 4 * (c & 1) : (D == 256 ? 2 * c : 0);
-      const int x = ((c & 1) << 1) | (c >> 1);         // row_of(t) ^ t of tokens 4c + i
-      const uint32_t vb = base + L::kV + 4 * c * L::kRow + (r ^ vturn) * (D / 16);
-      uint32_t w[4][kWords];
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) lds_words<kWords>(vb + (i ^ x) * L::kRow, w[i]);
-      uint32_t sc01[2], sc23[2];
-      constexpr int kGroups = D == 256 ? 2 : 1;
+        for (int e = 0; e < 4; ++e) p[e] = exp2_fast(t[ti][nt][e]);
+        l[nt][0] += p[0] + p[2];
+        l[nt][1] += p[1] + p[3];
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        uint32_t sw[1];
-        const int grp = D == 64 ? r >> 1 : (D == 128 ? r : 2 * r + g);
-        lds_words<1>(base + L::kVScale + grp * 16 + 4 * c, sw);
-        sc01[g] = e4m3x2_to_half2(sw[0]) & keep01;
-        sc23[g] = e4m3x2_to_half2(sw[0] >> 16) & keep23;
-      }
-#pragma unroll
-      for (int q = 0; q < kWords; ++q) {
-        constexpr uint32_t kLo = 0x0f0f0f0fu, kHi = 0xf0f0f0f0u;
-        uint32_t e01[4], d01[4], e23[4], d23[4];
-        fp4x8_to_half((w[0][q] & kLo) | ((w[1][q] << 4) & kHi), e01);  // even dims of tokens 0, 1
-        fp4x8_to_half(((w[0][q] >> 4) & kLo) | (w[1][q] & kHi), d01);  // odd dims
-        fp4x8_to_half((w[2][q] & kLo) | ((w[3][q] << 4) & kHi), e23);
-        fp4x8_to_half(((w[2][q] >> 4) & kLo) | (w[3][q] & kHi), d23);
-        const int g = D == 256 ? q >> 1 : 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t af[4] = {hmul2(e01[b], sc01[g]), hmul2(d01[b], sc01[g]), hmul2(e23[b], sc23[g]),
-                            hmul2(d23[b], sc23[g])};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(o[nt][4 * q + b], af, pb0[nt], pb1[nt]);
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = MmaOp<__half>::pack(p[2 * i], p[2 * i + 1]);
+          pb[ti][nt][i] = movmatrix_trans(hi);
+          pl[ti][nt][i] = 0;
+          if (kSplitP) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            pl[ti][nt][i] = movmatrix_trans(
+                MmaOp<__half>::pack(p[2 * i] - f.x, p[2 * i + 1] - f.y));
+          }
         }
       }
-    }
+    values(base, pb[0], pl[0], keep01[0], keep23[0]);
+    values(base + L::kBytes, pb[1], pl[1], keep01[1], keep23[1]);
   }
 };
 
-// Combines `n` states read through `get(k, m, l, o4)` for one float4 of O.
-struct Fp4Sum {
-  float m, l;
-  float4 o;
-};
-
-__device__ __forceinline__ void fp4_fold(Fp4Sum& acc, float m, float l, float4 o, float unit) {
-  const float top = fmaxf(acc.m, m);
-  const float a = exp2_fast((acc.m - top) * unit), b = exp2_fast((m - top) * unit);
-  acc.l = acc.l * a + l * b;
-  acc.o.x = acc.o.x * a + o.x * b;
-  acc.o.y = acc.o.y * a + o.y * b;
-  acc.o.z = acc.o.z * a + o.z * b;
-  acc.o.w = acc.o.w * a + o.w * b;
-  acc.m = top;
-}
-
-template <typename T>
-__device__ __forceinline__ void fp4_write(const DecodeFp4Args& a, int b, int qh, int d4,
-                                          const Fp4Sum& s) {
-  const float inv = s.l != 0.f ? a.v_scale / s.l : 0.f;
-  T* p = fp4_out_row<T>(a, b, qh) + d4 * 4;
-  p[0] = from_float<T>(s.o.x * inv);
-  p[1] = from_float<T>(s.o.y * inv);
-  p[2] = from_float<T>(s.o.z * inv);
-  p[3] = from_float<T>(s.o.w * inv);
-  if (d4 == 0 && a.lse != nullptr)
-    a.lse[static_cast<int64_t>(b) * a.hq + qh] = fp4_lse(a, s.m, s.l);
-}
-
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kPlain>
 __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
     paged_decode_fp4_kernel(const DecodeFp4Args a) {
   using S = Fp4Shape<D, NT>;
   constexpr int NCW = S::NCW, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int s_endpair[NCW];
-  __shared__ int s_abort;
   uint8_t* smem = smem_raw + ((128 - (smem_addr(smem_raw) & 127)) & 127);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kData);
   int* s_cum = reinterpret_cast<int*>(bars + NCW * NS);
+  int* s_len = s_cum + a.batch + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* full = bars + warp * NS;
-  if (warp == 0) fp4_build_prefix(a, s_cum, lane);
+  // Always a programmatic dependent: the CTA is placed while the kernel before
+  // it ends.  Without decode overlap it reads nothing before that one is done.
+  if (!a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 0) fp4_build_prefix(a, s_cum, s_len, lane);
   if (lane < NS) mbar_init(&full[lane], 1);
   fence_barrier_init();
-  if (threadIdx.x == 0) s_abort = 0;
   __syncthreads();
   // the merge kernel may be placed now; it waits for this grid to complete
   asm volatile("griddepcontrol.launch_dependents;");
@@ -588,39 +634,50 @@ __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
   // table and tiles outside each sequence's last page only.
   const int total = s_cum[a.batch] * a.hkv;
   const int W = total > 0 ? div_up(total, a.num_workers) : 0;
-  const int v = blockIdx.x * NCW + warp;
+  const int v = blockIdx.x * a.warps + warp;
   const int64_t first64 = static_cast<int64_t>(v) * W;
   const int first = first64 < total ? static_cast<int>(first64) : total;
   const int my_len = min(W, total - first);
-  const uint32_t ring = smem_addr(smem) + warp * NS * S::kTile;
+  const uint32_t ring = smem_addr(smem) + warp * NS * S::kUnit;
 
+  // Lane 2i + j of a window of 16 units holds the source of tile j of unit i
+  // (nullptr where there is none), one window ahead of the copies.
+  auto page_of = [&](int tile) {
+    return a.tpp_magic == 0 ? tile >> a.tpp_shift
+                            : static_cast<int>(__umulhi(static_cast<uint32_t>(tile), a.tpp_magic));
+  };
   auto tile_src = [&](int s, const uint8_t*& src, bool& tail) {
-    src = a.pool;
+    src = nullptr;
     tail = false;
     if (s >= my_len) return;
-    const TilePos p = locate(s_cum, a.batch, a.hkv, first + s);
-    const int page = p.t / a.tiles_per_page;
-    tail = page == (s_cum[p.b + 1] - s_cum[p.b] - 1) / a.tiles_per_page;
+    const TilePos p = fp4_locate(s_cum, a.batch, a.hkv, first + s);
+    const int tile = 2 * p.t + (lane & 1);
+    const int last = div_up(s_len[p.b], kFp4TileTokens) - 1;
+    if (tile > last) return;
+    const int page = page_of(tile);
+    tail = page == page_of(last);
     int64_t slot = a.page_table[static_cast<int64_t>(p.b) * a.pt_sb + page];
     if (slot < 0 || slot >= a.pool_pages) {
       report_status(HELM_DEV_BAD_PAGE);
       slot = 0;
     }
-    src = a.pool + ((slot * a.hkv + p.h) * a.tiles_per_page + (p.t - page * a.tiles_per_page)) *
-                       S::kTile;
+    src = a.pool +
+          ((slot * a.hkv + p.h) * a.tiles_per_page + (tile - page * a.tiles_per_page)) * S::kTile;
   };
-  // lane i holds the source of tile 32 * window + i, one window ahead
   const uint8_t *src_cur, *src_nxt;
   bool tail_cur, tail_nxt;
-  tile_src(lane, src_cur, tail_cur);
-  const bool opens = lane < NS && lane < my_len;
-  if (opens) {
-    mbar_arrive_expect_tx(&full[lane], S::kTile);
-    if (!tail_cur) bulk_load(ring + lane * S::kTile, src_cur, S::kTile, &full[lane]);
-  }
+  tile_src(lane >> 1, src_cur, tail_cur);
+  // the first NS units (2 NS <= 32 lanes), then the last-page tiles among them
+  unsigned have = __ballot_sync(0xffffffffu, src_cur != nullptr);
+  const int two = __popc(have >> (lane & 30) & 3u);
+  const bool opens = lane < 2 * NS && src_cur != nullptr;
+  const uint32_t open_dst = ring + (lane >> 1) * S::kUnit + (lane & 1) * S::kTile;
+  if (opens && (lane & 1) == 0) mbar_arrive_expect_tx(&full[lane >> 1], two * S::kTile);
+  __syncwarp();
+  if (opens && !tail_cur) bulk_load(open_dst, src_cur, S::kTile, &full[lane >> 1]);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (opens && tail_cur) bulk_load(ring + lane * S::kTile, src_cur, S::kTile, &full[lane]);
-  tile_src(32 + lane, src_nxt, tail_nxt);
+  if (opens && tail_cur) bulk_load(open_dst, src_cur, S::kTile, &full[lane >> 1]);
+  tile_src(16 + (lane >> 1), src_nxt, tail_nxt);
 
   // Pairs without tokens: zero output, LSE = -inf.
   for (int p = blockIdx.x; p < a.batch * a.hkv; p += gridDim.x) {
@@ -631,47 +688,54 @@ __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
     if (a.lse != nullptr && threadIdx.x < a.group)
       a.lse[static_cast<int64_t>(b) * a.hq + h * a.group + threadIdx.x] = -INFINITY;
   }
-  if (blockIdx.x * static_cast<int64_t>(NCW) * W >= total) return;  // whole CTA without work
-
-  Fp4Worker<T, D, NT> st;
-  TilePos pos;
-  if (my_len > 0) pos = locate(s_cum, a.batch, a.hkv, first);
+  Fp4Worker<T, D, NT, kPlain> st;
+  st.lane_offsets(lane);
   bool ok = true;
   int stage = 0, parity = 0;
-  for (int s = 0; s < my_len; ++s) {
-    if (pos.b != st.cur_b || pos.h != st.cur_h) {
-      if (st.cur_b >= 0) {
-        const Fp4Span ps = fp4_span(s_cum, a.hkv, W, total, st.cur_b, st.cur_h);
-        st.flush(a, ps.vf == ps.vl, v, lane);
+  for (int s = 0; s < my_len;) {
+    // the part of this warp's range that lies in one pair
+    const TilePos pos = fp4_locate(s_cum, a.batch, a.hkv, first + s);
+    st.cur_b = pos.b;
+    st.cur_h = pos.h;
+    st.reset();
+    st.load_q(a, pos.b, pos.h, lane);
+    const int units = s_cum[pos.b + 1] - s_cum[pos.b];
+    const int end = min(my_len, s + units - pos.t);
+    const int len = s_len[pos.b];
+    // units before `whole` need no checks: all of their tokens exist and count
+    const int whole = (kPlain || a.mask == nullptr) ? s + (len / kUnitTokens - pos.t) : s;
+    for (int tok0 = pos.t * kUnitTokens; s < end; ++s, tok0 += kUnitTokens) {
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&full[stage], parity))) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], parity));
+        if (!ok) break;
       }
-      st.cur_b = pos.b;
-      st.cur_h = pos.h;
-      st.cur_len = min(a.kv_lens[pos.b], (s_cum[pos.b + 1] - s_cum[pos.b]) * kFp4TileTokens);
-      st.reset();
-      st.load_q(a, pos.b, pos.h, lane);
+      const uint32_t at = ring + stage * S::kUnit;
+      if (s < whole)
+        st.template unit<true>(a, at, kUnitTokens, tok0, lane);
+      else
+        st.template unit<false>(a, at, min(kUnitTokens, len - tok0), tok0, lane);
+      __syncwarp();
+      const int nx = s + NS;  // the stage is read: its next unit
+      if ((nx & 15) == 0) {
+        src_cur = src_nxt;
+        have = __ballot_sync(0xffffffffu, src_cur != nullptr);
+        tile_src(nx + 16 + (lane >> 1), src_nxt, tail_nxt);
+      }
+      if (nx < my_len) {
+        if (lane == 0)
+          mbar_arrive_expect_tx(&full[stage], (have >> (2 * (nx & 15)) & 2u) ? S::kUnit : S::kTile);
+        __syncwarp();
+        if ((lane >> 1) == (nx & 15) && src_cur != nullptr)
+          bulk_load(at + (lane & 1) * S::kTile, src_cur, S::kTile, &full[stage]);
+      }
+      if (++stage == NS) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
-    if (!mbar_wait(&full[stage], parity)) ok = false;
-    if (__any_sync(0xffffffffu, !ok)) {
-      ok = false;
-      break;
-    }
-    const int tok0 = pos.t * kFp4TileTokens;
-    st.tile(a, ring + stage * S::kTile, min(kFp4TileTokens, st.cur_len - tok0), tok0, lane);
-    __syncwarp();
-    const int nx = s + NS;  // the stage is read: its next tile
-    if ((nx & 31) == 0) {
-      src_cur = src_nxt;
-      tile_src(nx + 32 + lane, src_nxt, tail_nxt);
-    }
-    if (nx < my_len && lane == (nx & 31)) {
-      mbar_arrive_expect_tx(&full[stage], S::kTile);
-      bulk_load(ring + stage * S::kTile, src_cur, S::kTile, &full[stage]);
-    }
-    advance(pos, s_cum, a.batch, a.hkv);
-    if (++stage == NS) {
-      stage = 0;
-      parity ^= 1;
-    }
+    if (!ok) break;
+    const Fp4Span ps = fp4_span(a, s_cum, W, st.cur_b, st.cur_h);
+    st.flush(a, ps.vf == ps.vl, v, lane);
   }
   // A wait that gave up leaves copies in flight into this CTA's shared memory:
   // wait (bounded) for those of this warp before it ends.
@@ -683,202 +747,199 @@ __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
         parity ^= 1;
       }
     }
-    if (lane == 0) s_abort = 1;
-  }
-  __syncthreads();
-  if (s_abort) return;
-  // ============ merge: as paged_decode_kernel, records over the idle ring =====
-  float* s_states = reinterpret_cast<float*>(smem);
-  int end_pair = -1;
-  if (st.cur_b >= 0) {
-    end_pair = st.cur_b * a.hkv + st.cur_h;
-    const Fp4Span ps = fp4_span(s_cum, a.hkv, W, total, st.cur_b, st.cur_h);
-    if (ps.vf == ps.vl) {
-      st.flush(a, true, v, lane);
-      end_pair = -1;
-    } else {
-      st.save(a, s_states + warp * S::kRec, lane);
-    }
-  }
-  if (lane == 0) s_endpair[warp] = end_pair;
-  __syncthreads();
-  constexpr int D4 = D / 4;
-  for (int w0 = 0; w0 < NCW;) {
-    const int p = s_endpair[w0];
-    int w1 = w0 + 1;
-    while (w1 < NCW && s_endpair[w1] == p) ++w1;
-    if (p >= 0) {
-      const int b = p / a.hkv, h = p - b * a.hkv;
-      const Fp4Span ps = fp4_span(s_cum, a.hkv, W, total, b, h);
-      const bool whole = ps.vf / NCW == ps.vl / NCW;  // the pair lies in this CTA
-      for (int e = threadIdx.x; e < a.group * D4; e += S::kThreads) {
-        const int hg = e / D4, d4 = e - hg * D4;
-        Fp4Sum acc = {kLowest, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-        for (int w = w0; w < w1; ++w) {
-          const float* rec = s_states + w * S::kRec;
-          fp4_fold(acc, rec[hg], rec[S::kHeads + hg],
-                   *reinterpret_cast<const float4*>(rec + 2 * S::kHeads + hg * D + d4 * 4),
-                   a.unit_log2);
-        }
-        if (whole && ps.last_continues) {
-          // the pair's last warp went on past it: its state for the pair is in
-          // the warp partials (written before the barrier above)
-          const int64_t slot = static_cast<int64_t>(ps.vl + p) * a.group + hg;
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot * 2));
-          fp4_fold(acc, ml.x, ml.y,
-                   __ldcg(reinterpret_cast<const float4*>(a.part_o + slot * D + d4 * 4)),
-                   a.unit_log2);
-        }
-        if (whole) {
-          fp4_write<T>(a, b, h * a.group + hg, d4, acc);
-        } else {
-          const int64_t slot = static_cast<int64_t>(blockIdx.x + p) * a.group + hg;
-          *reinterpret_cast<float4*>(a.cta_o + slot * D + d4 * 4) = acc.o;
-          if (d4 == 0)
-            *reinterpret_cast<float2*>(a.cta_ml + slot * 2) = make_float2(acc.m, acc.l);
-        }
-      }
-    }
-    w0 = w1;
   }
 }
 
-// Merges the pairs whose tiles were split across CTAs.  CTA (pair, chunk) owns
-// kMergeElems float4 elements; its half-warps take disjoint subsets of the
-// sources and meet in shared memory (see merge_split_pairs_kernel).
-template <typename T, int D, int NCW>
-__global__ void __launch_bounds__(kMergeThreads, 4) merge_fp4_kernel(const DecodeFp4Args a) {
+// Merges the pairs whose units were split across warps.  A CTA owns 32 places of
+// the row of one query head of one pair: eight threads cover them, the 32 groups
+// of eight take disjoint subsets of the sources, all loads in flight at once,
+// each against its own maximum, and meet in shared memory.  (Combining the warps
+// of a CTA in shared memory first was slower: that put 2.2 us behind the last
+// unit, the larger merge here costs less.)
+constexpr int kFp4MergeThreads = 256;
+constexpr int kFp4MergeCols = 8;  // float4 places of a CTA
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kFp4MergeThreads) merge_fp4_kernel(const DecodeFp4Args a) {
+  constexpr int kGroups = kFp4MergeThreads / kFp4MergeCols, kBatch = 5;
+  constexpr int kParts = 8;  // threads that add up the groups of one float4
   extern __shared__ int s_cum_m[];
-  __shared__ float s_st[kMergeGroups][6][kMergeElems];
+  __shared__ float4 s_acc[kGroups][kFp4MergeCols];
+  __shared__ float2 s_ml[kGroups];
   asm volatile("griddepcontrol.launch_dependents;");
-  const int p = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp == 0) fp4_build_prefix(a, s_cum_m, lane);
+  const int p = blockIdx.x, hg = blockIdx.y, col0 = blockIdx.z * kFp4MergeCols;
+  const int b = p / a.hkv, h = p - b * a.hkv, G = a.group;
+  // the lengths were there before the decode kernel's wait, hence before this
+  // kernel could be placed
+  if (threadIdx.x < 32) fp4_build_prefix(a, s_cum_m, nullptr, threadIdx.x);
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int total = s_cum_m[a.batch] * a.hkv;
-  if (total == 0) return;
-  const int W = div_up(total, a.num_workers);
-  const int b = p / a.hkv, h = p - b * a.hkv;
-  const Fp4Span ps = fp4_span(s_cum_m, a.hkv, W, total, b, h);
-  if (ps.tiles == 0 || ps.vf / NCW == ps.vl / NCW) return;  // not split across CTAs
-  const int vl_end = ps.last_continues ? ps.vl - 1 : ps.vl;
-  const int c0 = ps.vf / NCW, n_cta = vl_end / NCW - c0 + 1;
-  const int K = n_cta + (ps.last_continues ? 1 : 0);
-  const int G = a.group;
-  constexpr int D4 = D / 4;
-  const int el = lane & (kMergeElems - 1);
-  const int grp = warp * 2 + (lane >> 4);
-  const int e = blockIdx.y * kMergeElems + el;
-  const bool active = e < G * D4;
-  const int hg = active ? e / D4 : 0, d4 = active ? e - hg * D4 : 0;
-  Fp4Sum acc = {kLowest, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-  for (int k0 = grp; active && k0 < K; k0 += kMergeGroups * 2) {
-    float2 ml[2];
-    float4 o[2];
+  const int W = total > 0 ? div_up(total, a.num_workers) : 1;
+  const Fp4Span ps = fp4_span(a, s_cum_m, W, b, h);
+  const int K = s_cum_m[b + 1] == s_cum_m[b] || ps.vf == ps.vl ? 0 : ps.vl - ps.vf + 1;
+  // every thread waits, also those with nothing to merge: this grid must not
+  // complete before the decode kernel
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (K == 0) return;
+  const int64_t slot0 = static_cast<int64_t>(ps.vf + p) * G + hg;  // source k: k * G further
+  const int el = threadIdx.x % kFp4MergeCols, grp = threadIdx.x / kFp4MergeCols;
+  const float2* src_ml = reinterpret_cast<const float2*>(a.part_ml) + slot0;
+  const float4* src_o = reinterpret_cast<const float4*>(a.part_o) + slot0 * (D / 4) + col0 + el;
+  float top = kLowest, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = grp; k0 < K; k0 += kGroups * kBatch) {
+    float2 ml[kBatch];
+    float4 o[kBatch];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = k0 + i * kMergeGroups;
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = k0 + i * kGroups;
       ml[i] = make_float2(kLowest, 0.f);
       o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k < K) {
-        const bool cta_src = k < n_cta;
-        const int64_t slot = static_cast<int64_t>((cta_src ? c0 + k : ps.vl) + p) * G + hg;
-        ml[i] = __ldcg(reinterpret_cast<const float2*>((cta_src ? a.cta_ml : a.part_ml) + slot * 2));
-        o[i] = __ldcg(
-            reinterpret_cast<const float4*>((cta_src ? a.cta_o : a.part_o) + slot * D + d4 * 4));
+        const int64_t at = static_cast<int64_t>(k) * G;
+        ml[i] = __ldcg(src_ml + at);
+        o[i] = __ldcg(src_o + at * (D / 4));
       }
     }
+    float t = top;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fp4_fold(acc, ml[i].x, ml[i].y, o[i], a.unit_log2);
+    for (int i = 0; i < kBatch; ++i) t = fmaxf(t, ml[i].x);
+    const float f = exp2_fast((top - t) * a.unit_log2);
+    top = t;
+    sum *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float w = exp2_fast((ml[i].x - top) * a.unit_log2);
+      sum = fmaf(w, ml[i].y, sum);
+      acc.x = fmaf(w, o[i].x, acc.x);
+      acc.y = fmaf(w, o[i].y, acc.y);
+      acc.z = fmaf(w, o[i].z, acc.z);
+      acc.w = fmaf(w, o[i].w, acc.w);
+    }
   }
-  s_st[grp][0][el] = acc.m;
-  s_st[grp][1][el] = acc.l;
-  s_st[grp][2][el] = acc.o.x;
-  s_st[grp][3][el] = acc.o.y;
-  s_st[grp][4][el] = acc.o.z;
-  s_st[grp][5][el] = acc.o.w;
+  s_acc[grp][el] = acc;
+  if (el == 0) s_ml[grp] = make_float2(top, sum);
   __syncthreads();
-  if (threadIdx.x >= kMergeElems || !active) return;
-  Fp4Sum sum = {kLowest, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (threadIdx.x >= kFp4MergeCols * kParts) return;  // whole warps
+  const int e2 = threadIdx.x / kParts, part = threadIdx.x % kParts;
+  float2 ml[kGroups / kParts];
+  top = kLowest;
 #pragma unroll
-  for (int g = 0; g < kMergeGroups; ++g)
-    fp4_fold(sum, s_st[g][0][el], s_st[g][1][el],
-             make_float4(s_st[g][2][el], s_st[g][3][el], s_st[g][4][el], s_st[g][5][el]),
-             a.unit_log2);
-  fp4_write<T>(a, b, h * G + hg, d4, sum);
+  for (int i = 0; i < kGroups / kParts; ++i) {
+    ml[i] = s_ml[part + i * kParts];
+    top = fmaxf(top, ml[i].x);
+  }
+  top = warp_max_xor(top, 1, kParts / 2);
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kGroups / kParts; ++i) {
+    const float w = exp2_fast((ml[i].x - top) * a.unit_log2);
+    const float4 x = s_acc[part + i * kParts][e2];
+    sum = fmaf(w, ml[i].y, sum);
+    acc.x = fmaf(w, x.x, acc.x);
+    acc.y = fmaf(w, x.y, acc.y);
+    acc.z = fmaf(w, x.z, acc.z);
+    acc.w = fmaf(w, x.w, acc.w);
+  }
+  sum = warp_sum_xor(sum, 1, kParts / 2);
+  acc.x = warp_sum_xor(acc.x, 1, kParts / 2);
+  acc.y = warp_sum_xor(acc.y, 1, kParts / 2);
+  acc.z = warp_sum_xor(acc.z, 1, kParts / 2);
+  acc.w = warp_sum_xor(acc.w, 1, kParts / 2);
+  if (part != 0) return;
+  const int qh = h * G + hg, place = (col0 + e2) * 4;
+  const float inv = sum != 0.f ? a.v_scale / sum : 0.f;
+  T* out = fp4_out_row<T>(a, b, qh);
+  T* lo = out + fp4_state_dim<D>(place);
+  T* hi = out + fp4_state_dim<D>(place + 2);
+  lo[0] = from_float<T>(acc.x * inv);
+  lo[1] = from_float<T>(acc.y * inv);
+  hi[0] = from_float<T>(acc.z * inv);
+  hi[1] = from_float<T>(acc.w * inv);
+  if (place == 0 && a.lse != nullptr)
+    a.lse[static_cast<int64_t>(b) * a.hq + qh] = fp4_lse(a, top, sum);
 }
 
 // ----------------------------------------------------------------- host side --
-template <typename T, int D, int NT>
-cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_tiles, cudaStream_t stream) {
+template <typename T, int D, int NT, bool kPlain>
+cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_units, cudaStream_t stream) {
   using S = Fp4Shape<D, NT>;
   static unsigned long long configured = 0;  // one bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(configured & (1ull << dev))) {
-    e = cudaFuncSetAttribute(paged_decode_fp4_kernel<T, D, NT>,
+    e = cudaFuncSetAttribute(paged_decode_fp4_kernel<T, D, NT, kPlain>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(S::smem_bytes(kMaxBatch)));
     if (e != cudaSuccess) return e;
     if (dev < 64) configured |= 1ull << dev;
   }
-  const int64_t want = (max_tiles + S::NCW - 1) / S::NCW;
+  // one unit per warp where there are few: first over SMs, then over warps
+  const int sms = num_sms_current_device();
+  a.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S::NCW, max_units / sms)));
   const int grid = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(num_sms_current_device(), want)));
-  a.num_workers = grid * S::NCW;
+      std::max<int64_t>(1, std::min<int64_t>(sms, (max_units + a.warps - 1) / a.warps)));
+  a.num_workers = grid * a.warps;
+  a.early = decode_overlap_enabled() ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  cfg.numAttrs = 1;
   cfg.stream = stream;
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(S::kThreads);
+  cfg.blockDim = dim3(a.warps * 32);
   cfg.dynamicSmemBytes = S::smem_bytes(a.batch);
-  cfg.numAttrs = decode_overlap_enabled() ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, paged_decode_fp4_kernel<T, D, NT>, a);
+  e = cudaLaunchKernelEx(&cfg, paged_decode_fp4_kernel<T, D, NT, kPlain>, a);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.hkv),
-                     static_cast<unsigned>((a.group * (D / 4) + kMergeElems - 1) / kMergeElems));
-  cfg.blockDim = dim3(kMergeThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.hkv), static_cast<unsigned>(a.group),
+                     D / 4 / kFp4MergeCols);
+  cfg.blockDim = dim3(kFp4MergeThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(a.batch + 1) * sizeof(int);
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_fp4_kernel<T, D, S::NCW>, a);
+  return cudaLaunchKernelEx(&cfg, merge_fp4_kernel<T, D>, a);
+}
+
+template <typename T, int D>
+cudaError_t dispatch_decode_fp4_nt(const DecodeFp4Args& a, bool plain, int64_t units,
+                                   cudaStream_t s) {
+  if (a.group <= 8)
+    return plain ? launch_decode_fp4<T, D, 1, true>(a, units, s)
+                 : launch_decode_fp4<T, D, 1, false>(a, units, s);
+  return plain ? launch_decode_fp4<T, D, 2, true>(a, units, s)
+               : launch_decode_fp4<T, D, 2, false>(a, units, s);
 }
 
 template <typename T>
-cudaError_t dispatch_decode_fp4(int head_dim, const DecodeFp4Args& a, int64_t tiles,
+cudaError_t dispatch_decode_fp4(int head_dim, const DecodeFp4Args& a, bool plain, int64_t units,
                                 cudaStream_t s) {
-  const bool one = a.group <= 8;
   switch (head_dim) {
     case 64:
-      return one ? launch_decode_fp4<T, 64, 1>(a, tiles, s) : launch_decode_fp4<T, 64, 2>(a, tiles, s);
+      return dispatch_decode_fp4_nt<T, 64>(a, plain, units, s);
     case 128:
-      return one ? launch_decode_fp4<T, 128, 1>(a, tiles, s)
-                 : launch_decode_fp4<T, 128, 2>(a, tiles, s);
+      return dispatch_decode_fp4_nt<T, 128>(a, plain, units, s);
     default:
-      return one ? launch_decode_fp4<T, 256, 1>(a, tiles, s)
-                 : launch_decode_fp4<T, 256, 2>(a, tiles, s);
+      return dispatch_decode_fp4_nt<T, 256>(a, plain, units, s);
   }
 }
 
-// Workspace: warp partials and CTA partials, O then (m, l) of each, 256-byte
-// aligned regions.
+// Workspace: warp partials, O then (m, l), 256-byte aligned regions.
 struct Fp4Workspace {
-  int64_t o, ml, cta_o, cta_ml;
+  int64_t o, ml;
   Fp4Workspace(int batch, int hq, int hkv, int d) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t group = hq / hkv, pairs = static_cast<int64_t>(batch) * hkv;
-    const int64_t sms = num_sms_current_device();
-    const int64_t warps = (sms * 16 + pairs) * group, ctas = (sms + pairs) * group;
-    o = up(warps * d * 4);
-    ml = up(warps * 8);
-    cta_o = up(ctas * d * 4);
-    cta_ml = up(ctas * 8);
+    const int64_t slots = static_cast<int64_t>(num_sms_current_device()) * kFp4MaxWarps +
+                          static_cast<int64_t>(batch) * hkv;
+    o = up(slots * (hq / hkv) * d * 4);
+    ml = up(slots * (hq / hkv) * 8);
   }
-  int64_t total() const { return o + ml + cta_o + cta_ml; }
+  int64_t total() const { return o + ml; }
 };
 
 }  // namespace
@@ -947,29 +1008,32 @@ extern "C" int helm_paged_decode_attention_fp4(
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(w);
   a.part_ml = reinterpret_cast<float*>(w + ws.o);
-  a.cta_o = reinterpret_cast<float*>(w + ws.o + ws.ml);
-  a.cta_ml = reinterpret_cast<float*>(w + ws.o + ws.ml + ws.cta_o);
   a.batch = batch;
   a.hq = num_q_heads;
   a.hkv = num_kv_heads;
   a.group = group;
   a.page_size = page_size;
   a.tiles_per_page = static_cast<int>(tpp);
-  a.plain = mask == nullptr && !(softcap > 0.f) && scale > 0.f ? 1 : 0;
+  a.tpp_magic = 0;
+  a.tpp_shift = 0;
+  if ((tpp & (tpp - 1)) == 0)
+    while ((int64_t(1) << a.tpp_shift) < tpp) ++a.tpp_shift;
+  else  // rounded up: exact while x * (tpp - 1) < 2^32, and tpp * x <= 2^31 / 16 here
+    a.tpp_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + tpp - 1) / tpp);
+  const bool plain = mask == nullptr && !(softcap > 0.f) && scale > 0.f;
   a.score_scale = scale * k_scale;
   a.softcap = softcap;
   a.v_scale = v_scale;
-  a.unit_log2 = a.plain ? 1.f : kLog2e;
-  a.unit_ln = a.plain ? kLn2 : 1.f;
-  // bound on the tiles of the call: it sizes the grid
-  int64_t tiles = table_tiles;
-  if (max_kv_len_hint > 0)
-    tiles = std::min<int64_t>(tiles, (static_cast<int64_t>(max_kv_len_hint) + 15) / 16 * batch *
-                                         num_kv_heads);
+  a.unit_log2 = plain ? 1.f : kLog2e;
+  a.unit_ln = plain ? kLn2 : 1.f;
+  // bound on the units of the call: it sizes the grid
+  int64_t tokens = static_cast<int64_t>(max_pages) * page_size;
+  if (max_kv_len_hint > 0) tokens = std::min<int64_t>(tokens, max_kv_len_hint);
+  const int64_t units = (tokens + kUnitTokens - 1) / kUnitTokens * batch * num_kv_heads;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == HELM_DTYPE_BF16
-                            ? dispatch_decode_fp4<__nv_bfloat16>(head_dim, a, tiles, s)
-                            : dispatch_decode_fp4<__half>(head_dim, a, tiles, s);
+                            ? dispatch_decode_fp4<__nv_bfloat16>(head_dim, a, plain, units, s)
+                            : dispatch_decode_fp4<__half>(head_dim, a, plain, units, s);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return HELM_ERR_CUDA;
