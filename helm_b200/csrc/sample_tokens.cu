@@ -17,12 +17,21 @@
 // sizes give the same token.
 //
 // A row is held by one cluster, its logits in the CTAs' shared memory: HBM is
-// read once.  Each filter's last kept candidate is found by a histogram over
-// 2048 equal steps of the logit (counts and weights; steps equal in the logit
-// spread the atomics of a bell-shaped row, digits of its bit pattern would not),
-// then by ranking the candidates of the one bin that it falls in.  A bin of more
-// than 1024 candidates (all logits equal, huge outliers) is bisected instead.
+// read once.  A filter needs its last kept candidate.  A histogram of counts
+// over 2048 equal steps of the logit (equal steps spread a bell-shaped row over
+// the bins; digits of its bit pattern would not) says in which bin it falls:
+// exactly for top-k, and for top-p by an estimate from counts times the weight at
+// the bins' centres, good to a few bins (a window of 32 is kept around it).  Then
+//   few: when at most 1024 candidates lie in that bin (window) or above, they are
+//        sorted in one CTA, which finishes the row; the others are done;
+//   many: one pass in fp64 sums the weights above the window, per warp, and each
+//        bin's of the window; only the candidates of the bin that the sums point
+//        to are sorted.  The sums serve the draw as well.
+// Whatever neither can decide (more than 1024 equal logits at the cut, say) is
+// bisected over the order of candidates, pass by pass.
 #include <cooperative_groups.h>
+
+#include <cstddef>
 
 #include "common.cuh"
 
@@ -31,12 +40,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSampThreads = 1024;
+constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kSampBins = 2048;
-constexpr int kSampCand = 1024;              // candidates ranked against each other
+constexpr int kSampWindow = 32;              // bins around the estimate of top-p's cut
+constexpr int kSampList = 1024;              // candidates sorted in one CTA
 constexpr int kSampMaxVocab = 1 << 18;       // 2^18 weights of 2^44 stay below 2^63
-constexpr int kSampSliceBytes = 160 * 1024;  // logits held by a CTA
+constexpr int kSampSliceBytes = 160 * 1024;  // most logits a CTA can hold
+constexpr int kSampSliceGoal = 80 * 1024;    // two CTAs an SM: one loads while the other computes
 constexpr int kSampMaxCluster = 8;
 typedef unsigned long long u64;
 
@@ -79,32 +90,34 @@ __device__ const double kExp2Table[64] = {
     0x1.fa7c1819e90d8p+0,
 };
 
-// exp(x) in units of 2^-44, for x <= 0, rounded to nearest.  x = (64 m + j)
-// ln2/64 + r with |r| <= ln2/128, e^r by its series to r^4 (next term < 4e-14).
-__device__ __forceinline__ u64 weight_fixed(double x, const double* table) {
-  if (!(x > -31.0)) return 0;  // below half a unit (2^-45 = e^-31.2)
+// w = exp(x) in units of 2^-44 for -31.4 < x <= 0, given y = x * 64 / ln 2:
+// 2^(j/64) from the table, e^r = 2^(y/64 - k/64) by its series to the fourth
+// power (|r| <= ln2/128, next term < 4e-14), rounded to nearest by adding 2^52.
+// No branches: the caller's loop interleaves several of these chains, which is
+// what fp64's latency needs.
+__device__ __forceinline__ u64 weight_fixed(double y, const double* table) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the integer
-  const double k = fma(x, 0x1.71547652b82fep+6, kMagic);
+  constexpr double kStep = 0.0108304246962491454596;  // ln2 / 64
+  const double k = y + kMagic;
   const int n = static_cast<int>(__double_as_longlong(k));
-  const double kd = k - kMagic;
-  double r = fma(kd, -0x1.62e42fcp-7, x);
-  r = fma(kd, -0x1.7d1cf79abc9e4p-34, r);
-  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
+  const double r = y - (k - kMagic);
+  double p = fma(r, kStep * kStep * kStep * kStep / 24.0, kStep * kStep * kStep / 6.0);
+  p = fma(p, r, kStep * kStep / 2.0);
+  p = fma(p, r, kStep);
   p = fma(p, r, 1.0);
   p *= table[n & 63];
-  // times 2^(44 + floor(n / 64)), then rounded to an integer by adding 2^52
   p = __longlong_as_double(__double_as_longlong(p) +
                            (static_cast<long long>(44 + (n >> 6)) << 52));
-  const double y = p + 4503599627370496.0;
-  return static_cast<u64>(__double_as_longlong(y)) & 0xfffffffffffffull;
+  return static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
-// Order-preserving bits of a float (NaN was replaced; -0 counts as +0).
+// Order-preserving bits of a float (NaN was replaced; -0 counts as +0), and back.
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
 // Larger = earlier in the order of candidates.
@@ -112,218 +125,213 @@ __device__ __forceinline__ u64 order_of(float f, int index) {
   return (static_cast<u64>(order_key(f)) << 32) | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int off) { return __shfl_up_sync(0xffffffffu, v, off); }
-
 template <typename V, typename Op>
 __device__ __forceinline__ V warp_reduce(V v, Op op) {
 #pragma unroll
   for (int off = 16; off; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
+struct AddOp {
+  template <typename V>
+  __device__ __forceinline__ V operator()(V a, V b) const {
+    return a + b;
+  }
+};
 
-struct SampleShared {
+struct __align__(16) SampleShared {
   double table[64];
-  u64 warp_u64[kSampWarps];
-  uint32_t warp_u32[kSampWarps];
-  float warp_f32[2][kSampWarps];
+  float warp_max[kSampWarps], warp_min[kSampWarps];
+  u64 warp_a[kSampWarps], warp_b[kSampWarps];
+  double warp_d[kSampWarps];
   // published to the cluster
   float pub_max, pub_min;
-  u64 pub_mass;
-  uint32_t pub_count;
-  int pub_index;
-  uint32_t pub_cand;
-  // results of block-wide searches
-  int found_bin;
-  u64 found_above, found_order, found_mass;
-  uint32_t found_count;
-  int result;
-  uint32_t hist_count[kSampBins], hist_lo[kSampBins], hist_hi[kSampBins];
-  u64 cand_order[kSampCand], cand_weight[kSampCand];      // this CTA's
-  u64 all_order[kSampCand], all_weight[kSampCand];        // the cluster's
+  u64 pub_a, pub_b;
+  uint32_t pub_n;
+  // results, the same for every CTA of the cluster
+  int bin_k, bin_p;               // bins of the filters' last candidates (bin_p: estimate)
+  uint32_t upto_k, in_k, upto_w;  // candidates up to and in bin_k; up to the window's end
+  uint32_t win_lo[kSampWindow], win_hi[kSampWindow];  // weights of the window's bins
+  int win_bin;                    // the window's bin that the weights point to
+  u64 win_over;                   // weight above it
+  uint32_t list_n;        // rank 0: candidates in its list
+  u64 last, last_mass;    // rank 0: last kept candidate, weight up to it
+  __align__(16) uint32_t hist[kSampBins];  // read four at a time
+  u64 list[kSampList], weight[kSampList];
 };
+
+static_assert(offsetof(SampleShared, hist) % 16 == 0, "");
 
 template <typename T>
 struct Sampler {
+  static constexpr int kVec = 16 / sizeof(T);
   const SampleArgs& a;
   SampleShared& s;
-  const T* slice;
+  T* slice;
   cg::cluster_group cluster;
   int base, n;       // first index and number of logits of this CTA
+  int vecs;          // 16-byte groups of its slice (padded with -inf)
+  int ranks, rank, lane, warp;
   float top;         // largest logit of the row
-  double inv_temp;
+  double inv_temp, scale;  // z = (l - l_max) inv_temp, y = (l - l_max) scale
   float bin_scale;
+  float least_logit;  // below it weights round to 0
 
-  __device__ Sampler(const SampleArgs& a_, SampleShared& s_, const T* sl)
-      : a(a_), s(s_), slice(sl), cluster(cg::this_cluster()) {}
-
-  __device__ __forceinline__ float logit(int i) const {
-    const float f = to_float<T>(slice[i]);
-    return f == f ? f : -INFINITY;
+  __device__ Sampler(const SampleArgs& a_, SampleShared& s_, T* sl)
+      : a(a_), s(s_), slice(sl), cluster(cg::this_cluster()) {
+    lane = threadIdx.x & 31;
+    warp = threadIdx.x >> 5;
+    ranks = static_cast<int>(cluster.num_blocks());
+    rank = static_cast<int>(cluster.block_rank());
   }
+
   __device__ __forceinline__ u64 weight(float f) const {
-    if (f == top) return u64(1) << 44;
-    return weight_fixed((static_cast<double>(f) - static_cast<double>(top)) * inv_temp, s.table);
+    const u64 w = weight_fixed((static_cast<double>(f) - static_cast<double>(top)) * scale, s.table);
+    return f == top ? u64(1) << 44 : (f >= least_logit ? w : 0);  // -inf is below it
   }
   __device__ __forceinline__ int bin(float f) const {
     return max(0, min(kSampBins - 1, static_cast<int>((top - f) * bin_scale)));
   }
+  __device__ __forceinline__ void get(int vec, float (&f)[kVec]) const {
+    const uint4 raw = reinterpret_cast<const uint4*>(slice)[vec];
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = to_float<T>(e[i]);
+  }
+  // fn(value, index within the slice) for every logit of vectors v0, v0 + step ..
+  template <typename Fn>
+  __device__ __forceinline__ void each(int v0, int v1, int step, Fn fn) const {
+    for (int v = v0; v < v1; v += step) {
+      float f[kVec];
+      get(v, f);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) fn(f[i], v * kVec + i);
+    }
+  }
+  // A warp owns a contiguous run of vectors, its lanes take turns.
+  __device__ __forceinline__ int seg_vecs() const { return (vecs + kSampWarps - 1) / kSampWarps; }
+  __device__ __forceinline__ int seg_begin(int w) const { return min(vecs, w * seg_vecs()); }
 
-  // Block-wide then cluster-wide sums of (count, mass).
-  __device__ void cluster_sum(uint32_t& count, u64& mass) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto add32 = [](uint32_t x, uint32_t y) { return x + y; };
-    auto add64 = [](u64 x, u64 y) { return x + y; };
-    count = warp_reduce(count, add32);
-    mass = warp_reduce(mass, add64);
+  // Exclusive running sums over the block, thread by thread; total to all.
+  template <typename V>
+  __device__ __forceinline__ V block_scan(V v, V* warp_sums, V& total) {
+    V inc = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const V x = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += x;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    V w = lane < kSampWarps ? warp_sums[lane] : V(0), winc = w;
+#pragma unroll
+    for (int off = 1; off < kSampWarps; off <<= 1) {
+      const V x = __shfl_up_sync(0xffffffffu, winc, off);
+      if (lane >= off) winc += x;
+    }
+    total = __shfl_sync(0xffffffffu, winc, kSampWarps - 1);
+    const V before = __shfl_sync(0xffffffffu, winc - w, warp);
+    __syncthreads();
+    return before + inc - v;
+  }
+
+  // Sums of a and b over the cluster.
+  __device__ void cluster_sum(u64& x, u64& y) {
+    x = warp_reduce(x, AddOp());
+    y = warp_reduce(y, AddOp());
     if (lane == 0) {
-      s.warp_u32[warp] = count;
-      s.warp_u64[warp] = mass;
+      s.warp_a[warp] = x;
+      s.warp_b[warp] = y;
     }
     __syncthreads();
     if (warp == 0) {
-      count = warp_reduce(s.warp_u32[lane], add32);
-      mass = warp_reduce(s.warp_u64[lane], add64);
+      x = warp_reduce(lane < kSampWarps ? s.warp_a[lane] : u64(0), AddOp());
+      y = warp_reduce(lane < kSampWarps ? s.warp_b[lane] : u64(0), AddOp());
       if (lane == 0) {
-        s.pub_count = count;
-        s.pub_mass = mass;
+        s.pub_a = x;
+        s.pub_b = y;
       }
     }
     cluster.sync();
-    count = 0;
-    mass = 0;
-    for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-      count += *cluster.map_shared_rank(&s.pub_count, r);
-      mass += *cluster.map_shared_rank(&s.pub_mass, r);
+    x = y = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const SampleShared* o = cluster.map_shared_rank(&s, r);
+      x += o->pub_a;
+      y += o->pub_b;
     }
     cluster.sync();  // everyone has read before the words are used again
   }
 
-  // Candidates (by count) or weight (by mass) before and in each bin: the first
-  // bin whose inclusive sum reaches the target.  Needs the complete histogram.
-  __device__ void find_bin(bool by_mass, u64 target) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int kPer = kSampBins / kSampThreads;
-    uint32_t c[kPer];
-    u64 m[kPer], sum_c = 0, sum_m = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int bn = threadIdx.x * kPer + i;
-      c[i] = 0;
-      m[i] = 0;
-      for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-        const SampleShared* o = cluster.map_shared_rank(&s, r);
-        c[i] += o->hist_count[bn];
-        m[i] += (static_cast<u64>(o->hist_hi[bn]) << 32) + o->hist_lo[bn];
+  // Descending bitonic sort of list[0 .. size), a power of two, by this CTA.
+  __device__ void sort(int size) {
+    const int t = threadIdx.x;
+    for (int k = 2; k <= size; k <<= 1) {
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        if (t < size / 2) {
+          const int i = 2 * t - (t & (j - 1));
+          const u64 x = s.list[i], y = s.list[i + j];
+          if ((x < y) == ((i & k) == 0)) {
+            s.list[i] = y;
+            s.list[i + j] = x;
+          }
+        }
+        // pairs less than 64 apart stay within a warp's 64 entries
+        if (j > 32 || (j == 1 && k >= 64))
+          __syncthreads();
+        else
+          __syncwarp();
       }
-      sum_c += c[i];
-      sum_m += m[i];
-    }
-    const u64 mine = by_mass ? sum_m : sum_c, mine_m = sum_m;
-    u64 inc = mine, inc_m = mine_m;
-    for (int off = 1; off < 32; off <<= 1) {
-      const u64 x = shfl_up64(inc, off), y = shfl_up64(inc_m, off);
-      if (lane >= off) {
-        inc += x;
-        inc_m += y;
-      }
-    }
-    if (lane == 31) {
-      s.warp_u64[warp] = inc;
-      s.all_weight[warp] = inc_m;
-    }
-    if (threadIdx.x == 0) s.found_bin = -1;
-    __syncthreads();
-    u64 before = 0, before_m = 0;
-    for (int w = 0; w < warp; ++w) {
-      before += s.warp_u64[w];
-      before_m += s.all_weight[w];
-    }
-    u64 ex = before + inc - mine, ex_m = before_m + inc_m - mine_m;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const u64 q = by_mass ? m[i] : c[i];
-      if (ex < target && ex + q >= target) {
-        s.found_bin = threadIdx.x * kPer + i;
-        s.found_above = ex;        // in the target's unit
-        s.found_mass = ex_m;       // weight above the bin
-        s.found_count = c[i];
-      }
-      ex += q;
-      ex_m += m[i];
     }
     __syncthreads();
   }
 
-  // The order of the last candidate kept by a filter that keeps candidates
-  // until their count (or weight) reaches `target`; `mass` gets the weight of
-  // all candidates up to and including it.
-  __device__ u64 last_kept(bool by_mass, u64 target, u64& mass) {
-    find_bin(by_mass, target);
-    const int fb = s.found_bin;
-    const u64 above = s.found_above, above_m = s.found_mass;
-    const uint32_t in_bin = s.found_count;
-    if (fb >= 0 && in_bin <= kSampCand) {
-      if (threadIdx.x == 0) s.pub_cand = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kSampThreads) {
-        const float f = logit(i);
-        if (bin(f) == fb) {
-          const uint32_t at = atomicAdd(&s.pub_cand, 1u);
-          s.cand_order[at] = order_of(f, base + i);
-          s.cand_weight[at] = weight(f);
-        }
+  // Sends the candidates that `pick` selects to the list of rank 0 (counted
+  // before: they fit), which afterwards holds them in no particular order.
+  template <typename Pick>
+  __device__ void gather(Pick pick) {
+    SampleShared* home = cluster.map_shared_rank(&s, 0);
+    each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
+      if (f > -INFINITY && pick(f)) {
+        const uint32_t at = atomicAdd(&home->list_n, 1u);
+        if (at < kSampList) home->list[at] = order_of(f, base + i);
       }
-      cluster.sync();
-      uint32_t at = 0;
-      for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-        const SampleShared* o = cluster.map_shared_rank(&s, r);
-        const uint32_t m = o->pub_cand;
-        for (uint32_t i = threadIdx.x; i < m; i += kSampThreads) {
-          s.all_order[at + i] = o->cand_order[i];
-          s.all_weight[at + i] = o->cand_weight[i];
-        }
-        at += m;
-      }
-      cluster.sync();  // copied: the lists may be used again
-      if (threadIdx.x < at) {
-        const u64 me = s.all_order[threadIdx.x], w = s.all_weight[threadIdx.x];
-        u64 before = 0, before_m = 0;
-        for (uint32_t j = 0; j < at; ++j) {
-          const bool earlier = s.all_order[j] > me;
-          before += earlier ? 1 : 0;
-          before_m += earlier ? s.all_weight[j] : 0;
-        }
-        const u64 ex = above + (by_mass ? before_m : before);
-        const u64 q = by_mass ? w : 1;
-        if (ex < target && ex + q >= target) {
-          s.found_order = me;
-          s.found_above = above_m + before_m + w;
-        }
-      }
-      __syncthreads();
-      mass = s.found_above;
-      const u64 r = s.found_order;
-      __syncthreads();
-      return r;
+    });
+    cluster.sync();
+  }
+
+  // Rank 0: sorts its list, weighs it and leaves exclusive running sums in
+  // registers: entries 2t and 2t + 1 are this thread's.
+  __device__ void order_list(int count, u64 (&w)[2], u64 (&ex)[2], u64& total) {
+    int size = 64;
+    while (size < count) size <<= 1;
+    for (int i = count + threadIdx.x; i < size; i += kSampThreads) s.list[i] = 0;
+    __syncthreads();
+    sort(size);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = 2 * threadIdx.x + i;
+      w[i] = at < count ? weight(key_value(static_cast<uint32_t>(s.list[at] >> 32))) : 0;
     }
-    // bisection over the order itself: the largest order whose candidates (it
-    // and all earlier ones) reach the target
-    u64 lo = 0, hi = ~u64(0);  // reach(lo) holds, reach(hi) does not
-    u64 at_lo = 0;
+    ex[0] = block_scan(w[0] + w[1], s.warp_a, total);
+    ex[1] = ex[0] + w[0];
+  }
+
+  // The slow and general way: the order of the last candidate kept by a filter
+  // that keeps candidates until their count (or weight) reaches `target`, by
+  // bisection over the order itself.  `mass`: weight up to and including it.
+  __device__ u64 bisect(bool by_mass, u64 target, u64& mass) {
+    u64 lo = 0, hi = ~u64(0), at_lo = 0;  // the set from lo on reaches the target, from hi on not
     bool have = false;
     while (hi - lo > 1) {
       const u64 mid = lo + (hi - lo) / 2;
-      uint32_t c = 0;
-      u64 m = 0;
-      for (int i = threadIdx.x; i < n; i += kSampThreads) {
-        const float f = logit(i);
-        if (order_of(f, base + i) >= mid) {
+      u64 c = 0, m = 0;
+      each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
+        if (f > -INFINITY && order_of(f, base + i) >= mid) {
           ++c;
           m += weight(f);
         }
-      }
+      });
       cluster_sum(c, m);
-      if ((by_mass ? m : static_cast<u64>(c)) >= target) {
+      if ((by_mass ? m : c) >= target) {
         lo = mid;
         at_lo = m;
         have = true;
@@ -332,9 +340,8 @@ struct Sampler {
       }
     }
     if (!have) {  // nothing reaches it: everything is kept
-      uint32_t c = 0;
-      u64 m = 0;
-      for (int i = threadIdx.x; i < n; i += kSampThreads) m += weight(logit(i));
+      u64 c = 0, m = 0;
+      each(threadIdx.x, vecs, kSampThreads, [&](float f, int) { m += weight(f); });
       cluster_sum(c, m);
       at_lo = m;
     }
@@ -342,38 +349,214 @@ struct Sampler {
     return lo;
   }
 
-  __device__ void run(int row) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ranks = static_cast<int>(cluster.num_blocks());
-    const int rank = static_cast<int>(cluster.block_rank());
-    if (threadIdx.x < 64) s.table[threadIdx.x] = kExp2Table[threadIdx.x];
+  // Cluster-wide histogram of the candidates' logits, and the bins in which the
+  // filters' last candidates fall (the last bin where a filter keeps everything).
+  __device__ void histogram(int k, bool use_k, float p, bool use_p) {
+    each(threadIdx.x, vecs, kSampThreads, [&](float f, int) {
+      if (f > -INFINITY) atomicAdd(&s.hist[bin(f)], 1u);
+    });
+    cluster.sync();
+    constexpr int kPer = kSampBins / kSampThreads;
+    static_assert(kPer == 4, "");
+    const int b0 = threadIdx.x * kPer;
+    uint32_t c[kPer] = {0};
+#pragma unroll
+    for (int r = 0; r < kSampMaxCluster; ++r) {
+      if (r < ranks) {
+        const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s, r)->hist + b0);
+        c[0] += x.x;
+        c[1] += x.y;
+        c[2] += x.z;
+        c[3] += x.w;
+      }
+    }
+    if (threadIdx.x == 0) {
+      s.bin_k = s.bin_p = kSampBins - 1;
+      s.in_k = s.upto_k = 0xffffffffu;
+    }
+    const uint32_t uk = static_cast<uint32_t>(k);
+    uint32_t total;
+    const uint32_t ex = block_scan(c[0] + c[1] + c[2] + c[3],
+                                   reinterpret_cast<uint32_t*>(s.warp_a), total);
+    uint32_t before = ex;
+    if (use_k) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (before < uk && before + c[i] >= uk) {
+          s.bin_k = b0 + i;
+          s.in_k = c[i];
+          s.upto_k = before + c[i];
+        }
+        before += c[i];
+      }
+    }
+    if (use_p) {
+      // weights at the bins' centres (fp32: an estimate); with top-k the first k
+      const float step = bin_scale > 0.f ? static_cast<float>(inv_temp) / bin_scale : 0.f;
+      float m[kPer], sum = 0.f;
+      before = ex;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t count = use_k ? min(c[i], before < uk ? uk - before : 0u) : c[i];
+        m[i] = static_cast<float>(count) * (__expf(-(b0 + i + 0.5f) * step) + 1e-30f);
+        sum += m[i];
+        before += c[i];
+      }
+      float all;
+      float at = block_scan(sum, s.warp_min, all);
+      const float want = p * all;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (m[i] > 0.f && at < want && at + m[i] >= want) s.bin_p = b0 + i;
+        at += m[i];
+      }
+    }
+    __syncthreads();
+    if (use_p) {
+      const int end = window_begin() + kSampWindow - 1;
+      before = ex;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        before += c[i];
+        if (b0 + i == end) s.upto_w = before;
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ int window_begin() const {
+    return max(0, min(s.bin_p - kSampWindow / 2, kSampBins - kSampWindow));
+  }
+
+  // Weights of the whole row, per lane: its sum (total), what lies above bin lo
+  // (above) and of that what min-p keeps (kept); the weights of the bins lo ..
+  // lo + kSampWindow - 1 are added up in shared memory.
+  __device__ __forceinline__ void weigh(int lo, double least, u64& total, u64& above, u64& kept) {
+    if (threadIdx.x < kSampWindow) s.win_lo[threadIdx.x] = s.win_hi[threadIdx.x] = 0;
+    __syncthreads();
+    const int s1 = seg_begin(warp + 1);
+    each(seg_begin(warp) + lane, s1, 32, [&](float f, int) {
+      const u64 w = weight(f);
+      const int at = bin(f) - lo;
+      total += w;
+      above += at < 0 ? w : 0;
+      kept += at < 0 && (static_cast<double>(w) >= least || f == top) ? w : 0;
+      if (static_cast<unsigned>(at) < static_cast<unsigned>(kSampWindow) && w != 0) {
+        const uint32_t x = static_cast<uint32_t>(w);
+        const uint32_t old = atomicAdd(&s.win_lo[at], x);
+        const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + x < old ? 1u : 0u);
+        if (hi) atomicAdd(&s.win_hi[at], hi);
+      }
+    });
+  }
+
+  // After weigh() and a cluster barrier: the bin of the window in which the
+  // weight from the top reaches target, -1 if none; over: the weight above it.
+  __device__ int window_find(int lo, u64 above, u64 target, u64& over) {
+    if (threadIdx.x == 0) s.win_bin = -1;
+    __syncthreads();
+    if (warp == 0) {
+      u64 m = 0;
+      for (int r = 0; r < ranks; ++r) {
+        const SampleShared* o = cluster.map_shared_rank(&s, r);
+        m += (static_cast<u64>(o->win_hi[lane]) << 32) + o->win_lo[lane];
+      }
+      u64 inc = m;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += x;
+      }
+      const u64 ex = above + inc - m;
+      if (ex < target && ex + m >= target) {
+        s.win_bin = lo + lane;
+        s.win_over = ex;
+      }
+    }
+    static_assert(kSampWindow == 32, "");
+    __syncthreads();
+    over = s.win_over;
+    return s.win_bin;
+  }
+
+  // target of top-p in units of weight: kept while the weight before is below it
+  __device__ __forceinline__ static u64 top_p_target(float p, u64 of) {
+    const u64 t = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(of)));
+    return max(u64(1), min(of, t));
+  }
+  __device__ __forceinline__ static u64 draw_goal(float u, u64 whole) {
+    const u64 g = static_cast<u64>(fmax(static_cast<double>(u), 0.0) * static_cast<double>(whole));
+    return g >= whole ? whole - 1 : g;
+  }
+
+  // The general way for one CTA alone, over the row in global memory: sums of
+  // weights, bisected for top-p's last candidate and then for the drawn index.
+  template <typename Pred>
+  __device__ u64 row_sum(const T* src, Pred pred) {
+    u64 x = 0, sum;
+    for (int i = threadIdx.x; i < a.vocab; i += kSampThreads) {
+      const float f = to_float<T>(src[i]);
+      if (f == f && pred(f, i)) x += weight(f);
+    }
+    block_scan(x, s.warp_a, sum);
+    return sum;
+  }
+  __device__ void alone(int row, float p, double least, float u, u64 row_total) {
+    const T* src = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.row_stride;
+    const u64 target = top_p_target(p, row_total);
+    u64 lo = 0, hi = ~u64(0);
+    while (hi - lo > 1) {
+      const u64 mid = lo + (hi - lo) / 2;
+      const u64 m = row_sum(src, [&](float f, int i) { return order_of(f, i) >= mid; });
+      (m >= target ? lo : hi) = mid;
+    }
+    auto keep = [&](float f, int i) {
+      return order_of(f, i) >= lo && (static_cast<double>(weight(f)) >= least || f == top);
+    };
+    const u64 goal = draw_goal(u, row_sum(src, keep));
+    int first = -1, end = a.vocab - 1;  // the sum up to `end` exceeds the goal, up to `first` not
+    while (end - first > 1) {
+      const int mid = first + (end - first) / 2;
+      const u64 m = row_sum(src, [&](float f, int i) { return i <= mid && keep(f, i); });
+      (m > goal ? end : first) = mid;
+    }
+    if (threadIdx.x == 0) finish(row, end, to_float<T>(src[end]), row_total);
+  }
+
+  // The token is found: by the thread that holds it.
+  __device__ __forceinline__ void finish(int row, int index, float f, u64 total) {
+    a.ids[row] = index;
+    if (a.logprobs != nullptr) {
+      const double z =
+          f == top ? 0.0 : (static_cast<double>(f) - static_cast<double>(top)) * inv_temp;
+      a.logprobs[row] = static_cast<float>(z - log(static_cast<double>(total) * 0x1p-44));
+    }
+  }
+
+  __device__ void run(int row, float mx, float mn) {
     const float temp = a.temperature != nullptr ? a.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
-    inv_temp = greedy ? 1.0 : 1.0 / static_cast<double>(temp);
     const int k = greedy || a.top_k == nullptr ? 0 : a.top_k[row];
     const float p = greedy || a.top_p == nullptr ? 1.f : a.top_p[row];
     const float mp = greedy || a.min_p == nullptr ? 0.f : a.min_p[row];
+    const float u32 = a.uniforms[row];
     const bool use_k = k > 0 && k < a.vocab, use_p = p < 1.f;
+    if (threadIdx.x < 64) s.table[threadIdx.x] = kExp2Table[threadIdx.x];
+    for (int i = threadIdx.x; i < kSampBins; i += kSampThreads) s.hist[i] = 0;
+    if (threadIdx.x == 0) s.list_n = 0;
 
     // ---- the row's largest and smallest finite logit -------------------------
-    float mx = -INFINITY, mn = INFINITY;
-    for (int i = threadIdx.x; i < n; i += kSampThreads) {
-      const float f = logit(i);
-      mx = fmaxf(mx, f);
-      if (f > -INFINITY) mn = fminf(mn, f);
-    }
-    mx = warp_reduce(mx, [](float x, float y) { return fmaxf(x, y); });
-    mn = warp_reduce(mn, [](float x, float y) { return fminf(x, y); });
+    auto fmax_op = [](float x, float y) { return fmaxf(x, y); };
+    auto fmin_op = [](float x, float y) { return fminf(x, y); };
+    mx = warp_reduce(mx, fmax_op);
+    mn = warp_reduce(mn, fmin_op);
     if (lane == 0) {
-      s.warp_f32[0][warp] = mx;
-      s.warp_f32[1][warp] = mn;
+      s.warp_max[warp] = mx;
+      s.warp_min[warp] = mn;
     }
-    for (int i = threadIdx.x; i < kSampBins; i += kSampThreads)
-      s.hist_count[i] = s.hist_lo[i] = s.hist_hi[i] = 0;
     __syncthreads();
     if (warp == 0) {
-      mx = warp_reduce(s.warp_f32[0][lane], [](float x, float y) { return fmaxf(x, y); });
-      mn = warp_reduce(s.warp_f32[1][lane], [](float x, float y) { return fminf(x, y); });
+      mx = warp_reduce(lane < kSampWarps ? s.warp_max[lane] : -INFINITY, fmax_op);
+      mn = warp_reduce(lane < kSampWarps ? s.warp_min[lane] : INFINITY, fmin_op);
       if (lane == 0) {
         s.pub_max = mx;
         s.pub_min = mn;
@@ -383,8 +566,9 @@ struct Sampler {
     top = -INFINITY;
     mn = INFINITY;
     for (int r = 0; r < ranks; ++r) {
-      top = fmaxf(top, *cluster.map_shared_rank(&s.pub_max, r));
-      mn = fminf(mn, *cluster.map_shared_rank(&s.pub_min, r));
+      const SampleShared* o = cluster.map_shared_rank(&s, r);
+      top = fmaxf(top, o->pub_max);
+      mn = fminf(mn, o->pub_min);
     }
     if (top == -INFINITY) {  // nothing to draw from (the same for every CTA)
       if (rank == 0 && threadIdx.x == 0) {
@@ -394,130 +578,317 @@ struct Sampler {
       cluster.sync();
       return;
     }
+    inv_temp = greedy ? 1.0 : 1.0 / static_cast<double>(temp);
+    scale = 92.332482616893656877 * inv_temp;  // 64 / ln 2
     // bins span the finite logits, at most 64 T (weights below e^-64 vanish)
+    least_logit = fmaxf(top - 31.3f * (greedy ? 1.f : temp), -3.402823466e38f);
     const float span = fminf(top - mn, fmaxf(64.f * temp, 32.f));
     bin_scale = span > 0.f && span < INFINITY ? (kSampBins - 1) / span : 0.f;
-
-    // ---- weights of all candidates, and the histogram --------------------------
-    u64 total = 0;
-    const bool want_hist = use_k || use_p;
-    const bool want_total = a.logprobs != nullptr || use_p || (!use_k && !greedy);
-    if (want_hist || want_total) {
-      for (int i = threadIdx.x; i < n; i += kSampThreads) {
-        const float f = logit(i);
-        const u64 w = weight(f);
-        total += w;
-        if (want_hist) {
-          const int bn = bin(f);
-          atomicAdd(&s.hist_count[bn], 1u);
-          if (w != 0) {
-            const uint32_t lo = static_cast<uint32_t>(w);
-            const uint32_t old = atomicAdd(&s.hist_lo[bn], lo);
-            const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
-            if (hi) atomicAdd(&s.hist_hi[bn], hi);
-          }
-        }
-      }
-      uint32_t none = 0;
-      cluster_sum(none, total);  // its barriers also complete the histogram
-    }
-    u64 last = 0, mass = total;  // everything is kept
-    if (use_k) last = last_kept(false, static_cast<u64>(k), mass);
-    if (use_p) {
-      // kept while the weight before a candidate is below p * mass
-      const double want = static_cast<double>(p) * static_cast<double>(mass);
-      const u64 target = max(u64(1), min(mass, static_cast<u64>(ceil(want))));
-      u64 unused;
-      last = max(last, last_kept(true, target, unused));
-    }
     const double least = static_cast<double>(mp) * 17592186044416.0;  // min_p in units of 2^-44
 
+    // ---- where the filters cut -------------------------------------------------
+    bool few = false;
+    if (use_k || use_p) {
+      histogram(k, use_k, p, use_p);
+      few = (use_k ? s.upto_k : s.upto_w) <= kSampList;
+    }
+
+    // ---- weights of the row -----------------------------------------------------
+    const int s0 = seg_begin(warp), s1 = seg_begin(warp + 1);
+    u64 row_total = 0, above = 0;
+    if (few) {
+      // Rank 0 finishes the row.  It needs the row's sum for top-p alone and for
+      // the log probability.
+      if (a.logprobs != nullptr || !use_k) {
+        each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight(f); });
+        cluster_sum(row_total, above);
+      }
+      const int upto = use_k ? s.bin_k : window_begin() + kSampWindow - 1;
+      gather([&](float f) { return bin(f) <= upto; });
+      if (rank == 0) finish_few(row, k, use_k, p, use_p, least, u32, row_total);
+      return;  // rank 0 touches no other CTA's memory from here on
+    }
+    u64 last = 0;        // every candidate from this order on is kept
+    u64 warp_kept = 0;   // of this warp's run of vectors
+    bool known = true;   // warp_kept is right
+    if (greedy) {
+      if (a.logprobs != nullptr)
+        each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight(f); });
+      each(s0 + lane, s1, 32, [&](float f, int) { warp_kept += f == top ? 1 : 0; });
+      warp_kept = warp_reduce(warp_kept, AddOp());
+      if (a.logprobs != nullptr) cluster_sum(row_total, above);
+    } else if (!use_k && !use_p) {
+      each(s0 + lane, s1, 32, [&](float f, int) {
+        const u64 w = weight(f);
+        row_total += w;
+        warp_kept += static_cast<double>(w) >= least || f == top ? w : 0;
+      });
+      warp_kept = warp_reduce(warp_kept, AddOp());
+      cluster_sum(row_total, above);
+    } else {
+      // Many candidates.  top-k first: its bin is exact.
+      u64 mass = 0;
+      int lo = use_k ? min(s.bin_k, kSampBins - kSampWindow) : window_begin();
+      weigh(lo, least, row_total, above, warp_kept);
+      warp_kept = warp_reduce(warp_kept, AddOp());
+      cluster_sum(row_total, above);
+      mass = row_total;
+      int cut = -1;  // bin of the last kept candidate
+      if (use_k && s.in_k != 0xffffffffu) {
+        if (s.in_k <= kSampList) {
+          u64 over = above;
+          for (int b = lo; b < s.bin_k; ++b)  // (the window may begin before bin_k)
+            for (int r = 0; r < ranks; ++r) {
+              const SampleShared* o = cluster.map_shared_rank(&s, r);
+              over += (static_cast<u64>(o->win_hi[b - lo]) << 32) + o->win_lo[b - lo];
+            }
+          last = bin_last(s.bin_k, false, static_cast<u64>(k) - (s.upto_k - s.in_k), over, mass);
+          cut = s.bin_k;
+        } else {
+          last = bisect(false, static_cast<u64>(k), mass);
+          known = false;
+        }
+      }
+      if (use_p) {
+        if (use_k) {  // the sums were taken at top-k's bin: again at top-p's
+          cluster.sync();
+          lo = window_begin();
+          u64 again = 0;
+          above = warp_kept = 0;
+          weigh(lo, least, again, above, warp_kept);
+          warp_kept = warp_reduce(warp_kept, AddOp());
+          cluster_sum(again, above);
+          known = true;
+        }
+        const u64 target = top_p_target(p, mass);
+        u64 over = 0, m = 0, by_p = 0;
+        const int found = window_find(lo, above, target, over);
+        uint32_t in_bin = 0;
+        if (found >= 0)
+          for (int r = 0; r < ranks; ++r) in_bin += cluster.map_shared_rank(&s, r)->hist[found];
+        if (found >= 0 && in_bin <= kSampList) {
+          by_p = bin_last(found, true, target - over, over, m);
+          cut = found;
+        }
+        if (by_p == 0) {
+          by_p = bisect(true, target, m);
+          known = false;
+        }
+        if (by_p < last) known = false;  // equal weights at the border: top-k is the stricter one
+        last = max(last, by_p);
+      }
+      if (known && last != 0) {
+        // what is kept of the bins lo .. cut joins the sums
+        u64 more = 0;
+        each(s0 + lane, s1, 32, [&](float f, int i) {
+          const int b = bin(f);
+          if (b >= lo && b <= cut && f > -INFINITY && order_of(f, base + i) >= last) {
+            const u64 w = weight(f);
+            more += static_cast<double>(w) >= least || f == top ? w : 0;
+          }
+        });
+        warp_kept += warp_reduce(more, AddOp());
+      } else {
+        known = false;
+      }
+    }
+
     // ---- the draw: running sums in index order ---------------------------------
-    const int seg = (n + kSampThreads - 1) / kSampThreads * 32;  // of a warp, within the slice
-    const int s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
-    auto kept = [&](int i) -> u64 {
-      const float f = logit(i);
+    auto keep = [&](float f, int i) -> u64 {
       if (greedy) return f == top ? 1 : 0;
       if (last != 0 && order_of(f, base + i) < last) return 0;
       const u64 w = weight(f);
       return static_cast<double>(w) >= least || f == top ? w : 0;
     };
-    u64 sum = 0;
-    for (int i = s0 + lane; i < s1; i += 32) sum += kept(i);
-    sum = warp_reduce(sum, [](u64 x, u64 y) { return x + y; });
-    if (lane == 0) s.warp_u64[warp] = sum;
-    __syncthreads();
-    u64 before = 0, mine = 0;  // before this warp, within the CTA
-    for (int w = 0; w < kSampWarps; ++w) {
-      if (w < warp) before += s.warp_u64[w];
-      mine += s.warp_u64[w];
+    if (!known) {
+      u64 x = 0;
+      each(s0 + lane, s1, 32, [&](float f, int i) { x += keep(f, i); });
+      warp_kept = warp_reduce(x, AddOp());
     }
-    if (threadIdx.x == 0) s.pub_mass = mine;
+    __syncthreads();
+    if (lane == 0) s.warp_b[warp] = warp_kept;
+    __syncthreads();
+    u64 mine = lane < kSampWarps ? s.warp_b[lane] : 0, inc = mine;  // every warp: the CTA's warps
+#pragma unroll
+    for (int off = 1; off < kSampWarps; off <<= 1) {
+      const u64 x = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += x;
+    }
+    const u64 cta = __shfl_sync(0xffffffffu, inc, kSampWarps - 1);
+    if (threadIdx.x == 0) s.pub_a = cta;
     cluster.sync();
-    u64 whole = 0;
+    u64 before = 0, whole = 0;
     for (int r = 0; r < ranks; ++r) {
-      const u64 m = *cluster.map_shared_rank(&s.pub_mass, r);
+      const u64 m = cluster.map_shared_rank(&s, r)->pub_a;
       if (r < rank) before += m;
       whole += m;
     }
     // the token is the first whose running sum exceeds u * whole
-    const double u = greedy ? 0.0 : static_cast<double>(a.uniforms[row]);
-    u64 target = static_cast<u64>(fmax(u, 0.0) * static_cast<double>(whole));
-    if (target >= whole) target = whole - 1;
-    if (before <= target && before + sum > target) {  // in this warp's segment
-      u64 run_sum = before;
-      for (int i0 = s0; i0 < s1; i0 += 32) {
-        const int i = i0 + lane;
-        const u64 w = i < s1 ? kept(i) : 0;
-        u64 inc = w;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const u64 x = shfl_up64(inc, off);
-          if (lane >= off) inc += x;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run_sum + inc > target);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) {
-            a.ids[row] = base + i;
-            if (a.logprobs != nullptr) {
-              const float f = logit(i);
-              const double z = f == top ? 0.0
-                                        : (static_cast<double>(f) - static_cast<double>(top)) * inv_temp;
-              a.logprobs[row] =
-                  static_cast<float>(z - log(static_cast<double>(total) * 0x1p-44));
-            }
+    const u64 goal = greedy ? 0 : draw_goal(u32, whole);
+    if (before <= goal && before + cta > goal) {  // in this CTA: which warp's run of vectors?
+      const u64 ex = before + inc - mine;
+      const unsigned hit = __ballot_sync(0xffffffffu, lane < kSampWarps && ex <= goal && ex + mine > goal);
+      const int w = max(0, __ffs(hit) - 1);
+      u64 at = __shfl_sync(0xffffffffu, ex, w);
+      // that run again, spread over the whole CTA in index order
+      const int v0 = seg_begin(w), v1 = seg_begin(w + 1);
+      const int per = (v1 - v0 + kSampThreads - 1) / kSampThreads;
+      const int t0 = min(v1, v0 + static_cast<int>(threadIdx.x) * per), t1 = min(v1, t0 + per);
+      u64 x = 0;
+      each(t0, t1, 1, [&](float f, int i) { x += keep(f, i); });
+      u64 sum;
+      at += block_scan(x, s.warp_a, sum);
+      if (at <= goal && at + x > goal) {
+        bool found = false;
+        each(t0, t1, 1, [&](float f, int i) {
+          if (found) return;
+          at += keep(f, i);
+          if (at > goal) {
+            found = true;
+            finish(row, base + i, f, row_total);
           }
-          break;
-        }
-        run_sum += __shfl_sync(0xffffffffu, inc, 31);
+        });
       }
     }
     cluster.sync();  // no CTA leaves while another may read its shared memory
   }
+
+  // Rank 0, its list holding every candidate that may be kept: the row's token.
+  __device__ void finish_few(int row, int k, bool use_k, float p, bool use_p, double least, float u,
+                             u64 row_total) {
+    const int count = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kSampList)));
+    u64 w[2], ex[2], sum;
+    order_list(count, w, ex, sum);
+    // top-p's share is of the first k, or of the row where there is no top-k
+    u64 of = row_total;
+    if (use_k) {
+      if (threadIdx.x == 0) s.last_mass = sum;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (2 * static_cast<int>(threadIdx.x) + i == k) s.last_mass = ex[i];
+      __syncthreads();
+      of = s.last_mass;
+    }
+    const u64 target = use_p ? top_p_target(p, of) : ~u64(0);
+    if (!use_k && sum < target) {  // the estimate fell short by more than the window
+      alone(row, p, least, u, row_total);
+      return;
+    }
+    // what is kept, in index order: (index complemented, place in the list)
+    u64 key[2] = {0, 0};
+    float value[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = 2 * threadIdx.x + i;
+      const bool keep = at < count && (!use_k || at < k) && ex[i] < target &&
+                        (static_cast<double>(w[i]) >= least || w[i] == u64(1) << 44);
+      const u64 entry = at < count ? s.list[at] : 0;
+      value[i] = key_value(static_cast<uint32_t>(entry >> 32));
+      if (keep) key[i] = (entry << 32) | static_cast<u64>(at) | 0x80000000ull;
+      s.weight[at] = keep ? w[i] : 0;
+    }
+    const int kept_n = __syncthreads_count(key[0] != 0) + __syncthreads_count(key[1] != 0);
+    if (threadIdx.x == 0) s.pub_n = 0;
+    int size = 64;
+    while (size < kept_n) size <<= 1;
+    for (int i = threadIdx.x; i < size; i += kSampThreads) s.list[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (key[i] != 0) s.list[atomicAdd(&s.pub_n, 1u)] = key[i];
+    __syncthreads();
+    sort(size);  // larger = smaller index
+    u64 iw[2], iex[2], whole;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = 2 * threadIdx.x + i;
+      iw[i] = at < kept_n ? s.weight[s.list[at] & 0x7fffffffu] : 0;
+    }
+    iex[0] = block_scan(iw[0] + iw[1], s.warp_a, whole);
+    iex[1] = iex[0] + iw[0];
+    const u64 goal = draw_goal(u, whole);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (iex[i] <= goal && iex[i] + iw[i] > goal) {
+        const u64 entry = s.list[2 * threadIdx.x + i];
+        s.bin_k = static_cast<int>(entry & 0x7fffffffu);  // its place in the first order
+        s.bin_p = static_cast<int>(0xffffffffu - static_cast<uint32_t>(entry >> 32));
+      }
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) == s.bin_k / 2)
+      finish(row, s.bin_p, s.bin_k & 1 ? value[1] : value[0], row_total);
+  }
+
+  // The order of the last kept candidate within a bin of at most kSampList
+  // candidates, where `need` more (counted or weighed) are to be kept; mass =
+  // above + the bin's weight up to it.  0 when the bin does not hold enough.
+  __device__ u64 bin_last(int which, bool by_mass, u64 need, u64 above, u64& mass) {
+    if (rank == 0 && threadIdx.x == 0) s.list_n = 0;
+    cluster.sync();
+    gather([&](float f) { return bin(f) == which; });
+    if (rank == 0) {
+      const int count = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kSampList)));
+      u64 w[2], ex[2], sum;
+      order_list(count, w, ex, sum);
+      if (threadIdx.x == 0) s.last = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u64 at = 2 * threadIdx.x + i;
+        const bool here = by_mass ? ex[i] < need && ex[i] + w[i] >= need : at + 1 == need;
+        if (here && at < static_cast<u64>(count)) {
+          s.last = s.list[at];
+          s.last_mass = above + ex[i] + w[i];
+        }
+      }
+    }
+    cluster.sync();
+    const SampleShared* o = cluster.map_shared_rank(&s, 0);
+    const u64 last = o->last;
+    mass = o->last_mass;
+    cluster.sync();
+    return last;
+  }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kSampThreads, 1) sample_tokens_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kSampThreads, 2) sample_tokens_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(s_raw);
   T* slice = reinterpret_cast<T*>(s_raw + (sizeof(SampleShared) + 15) / 16 * 16);
   Sampler<T> job(a, s, slice);
-  const int rank = static_cast<int>(job.cluster.block_rank());
-  const int row = blockIdx.x / job.cluster.num_blocks();
-  job.base = min(a.vocab, rank * a.slice);
+  constexpr int kVec = Sampler<T>::kVec;
+  const int row = blockIdx.x / job.ranks;
+  job.base = min(a.vocab, job.rank * a.slice);
   job.n = min(a.slice, a.vocab - job.base);
+  job.vecs = (job.n + kVec - 1) / kVec;
   const T* src = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.row_stride + job.base;
-  constexpr int kVec = 16 / sizeof(T);
-  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    const int nv = job.n / kVec;
-    for (int i = threadIdx.x; i < nv; i += kSampThreads)
-      reinterpret_cast<uint4*>(slice)[i] = reinterpret_cast<const uint4*>(src)[i];
-    for (int i = nv * kVec + threadIdx.x; i < job.n; i += kSampThreads) slice[i] = src[i];
-  } else {
-    for (int i = threadIdx.x; i < job.n; i += kSampThreads) slice[i] = src[i];
+  // into shared memory, NaN as -inf and the last vector padded with it
+  float mx = -INFINITY, mn = INFINITY;
+  const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+#pragma unroll 4
+  for (int v = threadIdx.x; v < job.vecs; v += kSampThreads) {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+    if (aligned && (v + 1) * kVec <= job.n) {
+      raw = __ldg(reinterpret_cast<const uint4*>(src) + v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        e[i] = v * kVec + i < job.n ? src[v * kVec + i] : from_float<T>(-INFINITY);
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const float f = to_float<T>(e[i]);
+      if (f != f) e[i] = from_float<T>(-INFINITY);
+      mx = fmaxf(mx, f);  // NaN loses
+      if (f > -INFINITY) mn = fminf(mn, f);
+    }
+    reinterpret_cast<uint4*>(slice)[v] = raw;
   }
-  __syncthreads();
-  job.run(row);
+  job.run(row, mx, mn);
 }
 
 template <typename T>
@@ -527,17 +898,19 @@ cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   constexpr int kFixed = (sizeof(SampleShared) + 15) / 16 * 16;
+  static_assert(kFixed + kSampSliceBytes <= 227 * 1024, "");
   if (dev >= 64 || !(configured & (1ull << dev))) {
     e = cudaFuncSetAttribute(sample_tokens_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kFixed + kSampSliceBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) configured |= 1ull << dev;
   }
-  // CTAs of a row: as many as hold its logits; more while SMs would be idle
-  // and every CTA keeps a few thousand logits
+  // CTAs of a row: as many as hold its logits two to an SM (one to an SM where a
+  // cluster of eight leaves more); more while SMs would be idle and every CTA
+  // keeps a few thousand logits
   int ctas = 1;
   auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
-  while (ctas < kSampMaxCluster && static_cast<int64_t>(slice_of(ctas)) * sizeof(T) > kSampSliceBytes)
+  while (ctas < kSampMaxCluster && static_cast<int64_t>(slice_of(ctas)) * sizeof(T) > kSampSliceGoal)
     ctas *= 2;
   while (ctas < kSampMaxCluster && batch * ctas * 2 <= num_sms_current_device() &&
          slice_of(ctas) > 8192)
