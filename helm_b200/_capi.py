@@ -170,6 +170,12 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+# torch's own accessors behind torch.cuda.current_stream / current_device, without
+# the Python objects around them (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _stream_handle(device: torch.device, stream=None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream(device)
     return s.cuda_stream
@@ -660,21 +666,46 @@ def fp4_page_bytes(num_kv_heads: int, page_size: int, head_dim: int) -> int:
     return n
 
 
-def _check_fp4_pool(what: str, pool: torch.Tensor, hkv: int, page_size: int, d: int, dev) -> None:
-    if (pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[1] != hkv
-            or pool.shape[2] * 16 != page_size or pool.shape[3] != 18 * d
-            or not pool.is_contiguous() or pool.device != dev):
-        raise HelmError(f"{what}: pool must be a contiguous uint8 [pages, Hkv, page_size / 16, "
-                        f"18 * head_dim] tensor on {dev}")
+def _refuse(what: str, why: str):
+    raise HelmError(f"{what}: {why}")
 
 
-def _on(what: str, dev, **tensors) -> None:
-    """Every given tensor lives on the CUDA device `dev`."""
-    if dev.type != "cuda":
+def _device_of(what: str, t: torch.Tensor) -> int:
+    """Index of the CUDA device that t is on."""
+    idx = t.get_device()
+    if idx < 0:
         raise HelmError(f"{what} runs on CUDA tensors only")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise HelmError(f"{what}: {name} is on {t.device}, not on {dev}")
+    return idx
+
+
+def _same_device(what: str, idx: int, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != idx:
+            raise HelmError(f"{what}: a tensor is on {t.device}, not on cuda:{idx}")
+
+
+def _call(idx: int, fn, *args) -> int:
+    """fn(*args) with device idx current."""
+    if _current_device() == idx:
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
+
+
+def _stream_of(idx: int, stream) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is not None:
+        return _raw_stream(idx)
+    return torch.cuda.current_stream(idx).cuda_stream
+
+
+def _check_fp4_pool(what: str, pool: torch.Tensor, hkv: int, page_size: int, d: int) -> None:
+    shape = pool.shape
+    if (pool.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != hkv
+            or shape[2] * 16 != page_size or shape[3] != 18 * d or not pool.is_contiguous()):
+        _refuse(what, "pool must be a contiguous uint8 [pages, Hkv, page_size / 16, 18 * head_dim] "
+                      "tensor")
 
 
 def kv_append_fp4(*, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor,
@@ -687,44 +718,48 @@ def kv_append_fp4(*, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor,
     fp32 throughout.  q [N, Hq, D], k/v [N, Hkv, D] (unit dim stride, 16-byte
     aligned rows), cos/sin [N, D], slot_rows int64 [N] (-1 = skip; distinct),
     pool from fp4_pool, k_scale/v_scale the cache's scales (powers of two)."""
-    N, Hkv, D = k.shape
-    dev = k.device
-    _on("kv_append_fp4", dev, v=v, q=q, q_out=q_out, cos=cos, sin=sin, q_norm_w=q_norm_w,
-        k_norm_w=k_norm_w, slot_rows=slot_rows)
-    _check_fp4_pool("kv_append_fp4", pool, Hkv, page_size, D, dev)
-    if v.shape != k.shape or v.stride(2) != 1 or k.stride(2) != 1:
-        raise HelmError("kv_append_fp4: k and v must be [N, Hkv, D] with a unit dim stride")
+    what = "kv_append_fp4"
+    idx = _device_of(what, k)
+    _same_device(what, idx, v, pool, slot_rows, q, q_out, q_norm_w, k_norm_w, cos, sin)
+    shape, dt = k.shape, k.dtype
+    if len(shape) != 3:
+        _refuse(what, "k must be [N, Hkv, D]")
+    N, Hkv, D = shape
+    _check_fp4_pool(what, pool, Hkv, page_size, D)
+    ks, vs = k.stride(), v.stride()
+    if v.shape != shape or v.dtype is not dt or vs[2] != 1 or ks[2] != 1:
+        _refuse(what, "k and v must be [N, Hkv, D] of one dtype with a unit dim stride")
+    if slot_rows.dtype is not torch.int64 or slot_rows.shape != (N,) or not slot_rows.is_contiguous():
+        _refuse(what, "slot_rows must be contiguous int64 [N]")
     if (q is None) != (q_out is None):
-        raise HelmError("kv_append_fp4: q and q_out go together")
-    if q is not None and (q.shape[0] != N or q.shape[2] != D or q_out.shape != q.shape
-                          or q.stride(2) != 1 or q_out.stride(2) != 1):
-        raise HelmError("kv_append_fp4: q and q_out must be [N, Hq, D] with a unit dim stride")
+        _refuse(what, "q and q_out go together")
+    qp = qop = None
+    qst = qsh = qot = qoh = Hq = rs = 0
+    if q is not None:
+        qs, qos, qshape = q.stride(), q_out.stride(), q.shape
+        if (len(qshape) != 3 or qshape[0] != N or qshape[2] != D or q_out.shape != qshape
+                or qs[2] != 1 or qos[2] != 1 or q.dtype is not dt or q_out.dtype is not dt):
+            _refuse(what, "q and q_out must be [N, Hq, D] of k's dtype with a unit dim stride")
+        qp, qop, Hq = q.data_ptr(), q_out.data_ptr(), qshape[1]
+        qst, qsh, _ = qs
+        qot, qoh, _ = qos
     if (cos is None) != (sin is None):
-        raise HelmError("kv_append_fp4: cos and sin go together")
-    if cos is not None and (cos.shape != (N, D) or sin.shape != (N, D) or cos.stride(1) != 1
-                            or sin.stride() != cos.stride()):
-        raise HelmError("kv_append_fp4: cos and sin must be [N, D] with equal strides")
+        _refuse(what, "cos and sin go together")
+    if cos is not None:
+        rope = cos.stride()
+        if (cos.shape != (N, D) or sin.shape != (N, D) or rope[1] != 1 or sin.stride() != rope
+                or cos.dtype is not dt or sin.dtype is not dt):
+            _refuse(what, "cos and sin must be [N, D] of k's dtype with equal strides")
+        rs = rope[0]
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
-            raise HelmError("kv_append_fp4: norm weights must be contiguous [D]")
-    dt = k.dtype
-    for t in (v, q, q_out, q_norm_w, k_norm_w, cos, sin):
-        if t is not None and t.dtype != dt:
-            raise HelmError(f"kv_append_fp4: {t.dtype} where {dt} is used")
-    if slot_rows.dtype != torch.int64 or slot_rows.shape != (N,) or not slot_rows.is_contiguous():
-        raise HelmError("kv_append_fp4: slot_rows must be contiguous int64 [N]")
-    with _on_device(dev):
-        rc = lib().helm_kv_append_fp4(
-            _ptr(q), q.stride(0) if q is not None else 0, q.stride(1) if q is not None else 0,
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-            _ptr(q_norm_w), _ptr(k_norm_w), eps,
-            _ptr(cos), _ptr(sin), cos.stride(0) if cos is not None else 0,
-            _ptr(q_out), q_out.stride(0) if q is not None else 0,
-            q_out.stride(1) if q is not None else 0,
-            pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(), N,
-            q.shape[1] if q is not None else 0, Hkv, D, page_size, helm_dtype(dt),
-            k_scale, v_scale, _stream_handle(dev, stream))
-    _check(rc, "helm_kv_append_fp4")
+        if w is not None and (w.shape != (D,) or w.dtype is not dt or not w.is_contiguous()):
+            _refuse(what, "norm weights must be contiguous [D] of k's dtype")
+    rc = _call(idx, (_lib or lib()).helm_kv_append_fp4, qp, qst, qsh, k.data_ptr(), ks[0], ks[1],
+               v.data_ptr(), vs[0], vs[1], _ptr(q_norm_w), _ptr(k_norm_w), eps, _ptr(cos),
+               _ptr(sin), rs, qop, qot, qoh, pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(),
+               N, Hq, Hkv, D, page_size, helm_dtype(dt), k_scale, v_scale, _stream_of(idx, stream))
+    if rc:
+        _check(rc, "helm_kv_append_fp4")
 
 
 def gather_kv_rows_fp4(pool: torch.Tensor, slot_rows: torch.Tensor, *, page_size: int,
@@ -733,30 +768,35 @@ def gather_kv_rows_fp4(pool: torch.Tensor, slot_rows: torch.Tensor, *, page_size
                        v_out: Optional[torch.Tensor] = None, stream=None):
     """K, V [N, Hkv, D] in `dtype`: the values of the pool rows slot_rows
     (int64 [N]; a negative row gives zeros).  k_out / v_out may be strided."""
-    dev = pool.device
-    _on("gather_kv_rows_fp4", dev, slot_rows=slot_rows, k_out=k_out, v_out=v_out)
+    what = "gather_kv_rows_fp4"
+    idx = _device_of(what, pool)
+    _same_device(what, idx, slot_rows, k_out, v_out)
     if pool.dim() != 4 or pool.shape[3] % 18:
-        raise HelmError("gather_kv_rows_fp4: pool is not a pool of 4-bit pages")
-    Hkv, D = pool.shape[1], pool.shape[3] // 18
-    _check_fp4_pool("gather_kv_rows_fp4", pool, Hkv, page_size, D, dev)
-    if slot_rows.dtype != torch.int64 or slot_rows.dim() != 1 or not slot_rows.is_contiguous():
-        raise HelmError("gather_kv_rows_fp4: slot_rows must be contiguous int64 [N]")
-    shape = (slot_rows.shape[0], Hkv, D)
-    with _on_device(dev):
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype, device=dev)
-        if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=dev)
-        for t in (k_out, v_out):
-            if t.shape != shape or t.dtype != dtype or t.stride(2) != 1:
-                raise HelmError("gather_kv_rows_fp4: outputs must be [N, Hkv, D] in dtype with a "
-                                "unit dim stride")
-        rc = lib().helm_gather_kv_rows_fp4(
-            pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(), k_out.data_ptr(),
-            k_out.stride(0), k_out.stride(1), v_out.data_ptr(), v_out.stride(0), v_out.stride(1),
-            shape[0], Hkv, D, page_size, helm_dtype(dtype), k_scale, v_scale,
-            _stream_handle(dev, stream))
-    _check(rc, "helm_gather_kv_rows_fp4")
+        _refuse(what, "pool is not a pool of 4-bit pages")
+    pages, Hkv, _, d18 = pool.shape
+    D = d18 // 18
+    _check_fp4_pool(what, pool, Hkv, page_size, D)
+    if slot_rows.dtype is not torch.int64 or slot_rows.dim() != 1 or not slot_rows.is_contiguous():
+        _refuse(what, "slot_rows must be contiguous int64 [N]")
+    N = slot_rows.shape[0]
+    if k_out is None:
+        k_out = torch.empty((N, Hkv, D), dtype=dtype, device=pool.device)
+        if stream is not None:
+            k_out.record_stream(stream)
+    if v_out is None:
+        v_out = torch.empty((N, Hkv, D), dtype=dtype, device=pool.device)
+        if stream is not None:
+            v_out.record_stream(stream)
+    ks, vs, shape = k_out.stride(), v_out.stride(), (N, Hkv, D)
+    if (k_out.shape != shape or v_out.shape != shape or k_out.dtype is not dtype
+            or v_out.dtype is not dtype or ks[2] != 1 or vs[2] != 1):
+        _refuse(what, "outputs must be [N, Hkv, D] in dtype with a unit dim stride")
+    rc = _call(idx, (_lib or lib()).helm_gather_kv_rows_fp4, pool.data_ptr(), pages,
+               slot_rows.data_ptr(), k_out.data_ptr(), ks[0], ks[1], v_out.data_ptr(), vs[0],
+               vs[1], N, Hkv, D, page_size, helm_dtype(dtype), k_scale, v_scale,
+               _stream_of(idx, stream))
+    if rc:
+        _check(rc, "helm_gather_kv_rows_fp4")
     return k_out, v_out
 
 
@@ -776,50 +816,59 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
     [B]; mask additive [B or 1, T] with T >= max(kv_lens), -inf excludes a key.
     Returns (out [B, Hq, D] in q.dtype, lse fp32 [B, Hq] or None).
     """
-    dev = q.device
-    _on("paged_decode_attention_fp4", dev, page_table=page_table, kv_lens=kv_lens, mask=mask,
-        out=out, lse=lse)
-    B, Hq, D = q.shape
-    _check_fp4_pool("paged_decode_attention_fp4", pool, num_kv_heads, page_size, D, dev)
-    if q.stride(2) != 1:
-        raise HelmError("q must have a unit stride on the head dim")
-    if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32:
-        raise HelmError("page_table and kv_lens must be int32")
-    if (page_table.dim() != 2 or page_table.shape[0] != B or page_table.stride(1) != 1
-            or kv_lens.shape != (B,) or not kv_lens.is_contiguous()):
-        raise HelmError("page_table must be [B, max_pages] with contiguous rows, kv_lens [B]")
+    what = "paged_decode_attention_fp4"
+    idx = _device_of(what, q)
+    _same_device(what, idx, pool, page_table, kv_lens, mask, out, lse)
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3:
+        _refuse(what, "q must be [B, Hq, D]")
+    B, Hq, D = shape
+    qs = q.stride()
+    if qs[2] != 1:
+        _refuse(what, "q must have a unit stride on the head dim")
+    _check_fp4_pool(what, pool, num_kv_heads, page_size, D)
+    i32, tshape, ts = torch.int32, page_table.shape, page_table.stride()
+    if page_table.dtype is not i32 or len(tshape) != 2 or tshape[0] != B or ts[1] != 1:
+        _refuse(what, "page_table must be int32 [B, max_pages] with contiguous rows")
+    if kv_lens.dtype is not i32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
+        _refuse(what, "kv_lens must be contiguous int32 [B]")
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:
-        raise HelmError("out must be [B, Hq, D] in the query dtype, unit dim stride")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq)
-                            or not lse.is_contiguous()):
-        raise HelmError("lse must be contiguous fp32 [B, Hq]")
+        out = torch.empty(shape, dtype=dt, device=q.device)
+        if stream is not None:
+            out.record_stream(stream)
+    os_ = out.stride()
+    if out.dtype is not dt or out.shape != shape or os_[2] != 1:
+        _refuse(what, "out must be [B, Hq, D] in the query dtype, unit dim stride")
+    lse_ptr = None
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous():
+            _refuse(what, "lse must be contiguous fp32 [B, Hq]")
+        lse_ptr = lse.data_ptr()
     mask_ptr, mask_dt, mask_sb = None, 0, 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[0] not in (1, B):
-            raise HelmError("mask must be [B or 1, T]")
+            _refuse(what, "mask must be [B or 1, T]")
         if mask.stride(1) != 1:
             mask = mask.contiguous()
         mask_ptr, mask_dt = mask.data_ptr(), helm_dtype(mask.dtype)
         mask_sb = mask.stride(0) if mask.shape[0] > 1 else 0
-    key = (dev.index, B, Hq, num_kv_heads, D)
-    with _on_device(dev):
-        nbytes = _fp4_ws_bytes.get(key)
-        if nbytes is None:
-            nbytes = _fp4_ws_bytes[key] = int(
-                lib().helm_paged_decode_fp4_workspace_bytes(B, Hq, num_kv_heads, D))
-        # scratch of this call alone: two captured graphs, or two streams, share none
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        if stream is not None:
-            ws.record_stream(stream)
-        rc = lib().helm_paged_decode_attention_fp4(
-            q.data_ptr(), q.stride(0), q.stride(1), pool.data_ptr(), pool.shape[0],
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(),
-            mask_ptr, mask_dt, mask_sb, out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
-            ws.data_ptr(), nbytes, B, Hq, num_kv_heads, D, page_size, helm_dtype(q.dtype), scale,
-            softcap or 0.0, k_scale, v_scale, max_kv_len_hint, _stream_handle(dev, stream))
-    _check(rc, "helm_paged_decode_attention_fp4")
+    L = _lib or lib()
+    key = (idx, B, Hq, num_kv_heads, D)
+    nbytes = _fp4_ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = _fp4_ws_bytes[key] = int(
+            _call(idx, L.helm_paged_decode_fp4_workspace_bytes, B, Hq, num_kv_heads, D))
+    # scratch of this call alone: two captured graphs, or two streams, share none
+    ws = pool.new_empty(nbytes)
+    if stream is not None:
+        ws.record_stream(stream)
+    rc = _call(idx, L.helm_paged_decode_attention_fp4, q.data_ptr(), qs[0], qs[1], pool.data_ptr(),
+               pool.shape[0], page_table.data_ptr(), ts[0], tshape[1], kv_lens.data_ptr(),
+               mask_ptr, mask_dt, mask_sb, out.data_ptr(), os_[0], os_[1], lse_ptr, ws.data_ptr(),
+               nbytes, B, Hq, num_kv_heads, D, page_size, helm_dtype(dt), scale, softcap or 0.0,
+               k_scale, v_scale, max_kv_len_hint, _stream_of(idx, stream))
+    if rc:
+        _check(rc, "helm_paged_decode_attention_fp4")
     return out, lse
 
 
@@ -841,46 +890,51 @@ def build_step_tables(past_lens: torch.Tensor, new_lens: torch.Tensor, page_tabl
     Returns (kv_lens [B], cu_tokens [B + 1], seq_ids, positions int32 [num_rows],
     slot_rows int64 [num_rows]); kv_lens may be past_lens itself.
     """
-    dev = past_lens.device
-    _on("build_step_tables", dev, new_lens=new_lens, page_table=page_table, free_pages=free_pages,
-        free_count=free_count, free_count_out=free_count_out, kv_lens=kv_lens,
-        cu_tokens=cu_tokens, seq_ids=seq_ids, positions=positions, slot_rows=slot_rows)
-    B = past_lens.shape[0]
+    what = "build_step_tables"
+    idx = _device_of(what, past_lens)
     i32 = torch.int32
+    if past_lens.dtype is not i32 or past_lens.dim() != 1:
+        _refuse(what, "past_lens must be int32 [B]")
+    B = past_lens.shape[0]
+    new = past_lens.new_empty
     if free_count_out is None:
         free_count_out = free_count
+    made = []  # what this call allocates
     if kv_lens is None:
-        kv_lens = torch.empty(B, dtype=i32, device=dev)
+        made.append(kv_lens := new(B))
     if cu_tokens is None:
-        cu_tokens = torch.empty(B + 1, dtype=i32, device=dev)
+        made.append(cu_tokens := new(B + 1))
     if seq_ids is None:
-        seq_ids = torch.empty(num_rows, dtype=i32, device=dev)
+        made.append(seq_ids := new(num_rows))
     if positions is None:
-        positions = torch.empty(num_rows, dtype=i32, device=dev)
+        made.append(positions := new(num_rows))
     if slot_rows is None:
-        slot_rows = torch.empty(num_rows, dtype=torch.int64, device=dev)
-    for name, t, n, dt in (("past_lens", past_lens, B, i32), ("new_lens", new_lens, B, i32),
-                           ("free_count", free_count, 1, i32),
-                           ("free_count_out", free_count_out, 1, i32),
-                           ("kv_lens", kv_lens, B, i32), ("cu_tokens", cu_tokens, B + 1, i32),
-                           ("seq_ids", seq_ids, num_rows, i32),
-                           ("positions", positions, num_rows, i32),
-                           ("slot_rows", slot_rows, num_rows, torch.int64),
-                           ("free_pages", free_pages, free_pages.shape[0], i32)):
-        if t.dtype != dt or t.shape != (n,) or not t.is_contiguous():
-            raise HelmError(f"build_step_tables: {name} must be contiguous {dt} [{n}]")
-    if (page_table.dtype != i32 or page_table.dim() != 2 or page_table.shape[0] != B
-            or page_table.stride(1) != 1):
-        raise HelmError("build_step_tables: page_table must be int32 [B, max_pages] with "
-                        "contiguous rows")
-    with _on_device(dev):
-        rc = lib().helm_build_step_tables(
-            past_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-            page_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
-            free_count_out.data_ptr(), kv_lens.data_ptr(), cu_tokens.data_ptr(),
-            seq_ids.data_ptr(), positions.data_ptr(), slot_rows.data_ptr(), B, page_size, num_rows,
-            _stream_handle(dev, stream))
-    _check(rc, "helm_build_step_tables")
+        made.append(slot_rows := new(num_rows, dtype=torch.int64))
+    if stream is not None:
+        for t in made:
+            t.record_stream(stream)
+    _same_device(what, idx, new_lens, page_table, free_pages, free_count, free_count_out, kv_lens,
+                 cu_tokens, seq_ids, positions, slot_rows)
+    one, each, rows = (1,), (B,), (num_rows,)
+    for t, n in ((past_lens, each), (new_lens, each), (kv_lens, each), (cu_tokens, (B + 1,)),
+                 (free_count, one), (free_count_out, one), (seq_ids, rows), (positions, rows)):
+        if t.dtype is not i32 or t.shape != n or not t.is_contiguous():
+            _refuse(what, "lengths, counts, cu_tokens, seq_ids and positions must be contiguous "
+                          "int32 [B], [1], [B + 1], [num_rows] and [num_rows]")
+    if slot_rows.dtype is not torch.int64 or slot_rows.shape != rows or not slot_rows.is_contiguous():
+        _refuse(what, "slot_rows must be contiguous int64 [num_rows]")
+    if free_pages.dtype is not i32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        _refuse(what, "free_pages must be contiguous int32 [capacity]")
+    tshape, ts = page_table.shape, page_table.stride()
+    if page_table.dtype is not i32 or len(tshape) != 2 or tshape[0] != B or ts[1] != 1:
+        _refuse(what, "page_table must be int32 [B, max_pages] with contiguous rows")
+    rc = _call(idx, (_lib or lib()).helm_build_step_tables, past_lens.data_ptr(),
+               new_lens.data_ptr(), page_table.data_ptr(), ts[0], tshape[1], free_pages.data_ptr(),
+               free_pages.shape[0], free_count.data_ptr(), free_count_out.data_ptr(),
+               kv_lens.data_ptr(), cu_tokens.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(),
+               slot_rows.data_ptr(), B, page_size, num_rows, _stream_of(idx, stream))
+    if rc:
+        _check(rc, "helm_build_step_tables")
     return kv_lens, cu_tokens, seq_ids, positions, slot_rows
 
 
@@ -895,25 +949,27 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
     logit.  Returns ids int64 [B] (-1: nothing to draw from); logprobs fp32 [B]
     gets the tokens' log softmax(l / T).  include/helm_b200.h has the definition.
     """
-    dev = logits.device
-    _on("sample_tokens", dev, uniforms=uniforms, temperature=temperature, top_k=top_k,
-        top_p=top_p, min_p=min_p, out=out, logprobs=logprobs)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise HelmError("sample_tokens: logits must be [B, V] with a unit inner stride")
-    B, V = logits.shape
-    for name, t, dt in (("uniforms", uniforms, torch.float32),
-                        ("temperature", temperature, torch.float32),
-                        ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                        ("min_p", min_p, torch.float32), ("out", out, torch.int64),
-                        ("logprobs", logprobs, torch.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
-            raise HelmError(f"sample_tokens: {name} must be contiguous {dt} [{B}]")
+    what = "sample_tokens"
+    idx = _device_of(what, logits)
+    _same_device(what, idx, uniforms, temperature, top_k, top_p, min_p, out, logprobs)
+    shape, ls = logits.shape, logits.stride()
+    if len(shape) != 2 or ls[1] != 1:
+        _refuse(what, "logits must be [B, V] with a unit inner stride")
+    B, V = shape
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=dev)
-    with _on_device(dev):
-        rc = lib().helm_sample_tokens(
-            logits.data_ptr(), logits.stride(0), helm_dtype(logits.dtype), uniforms.data_ptr(),
-            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(),
-            _ptr(logprobs), B, V, _stream_handle(dev, stream))
-    _check(rc, "helm_sample_tokens")
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+        if stream is not None:
+            out.record_stream(stream)
+    f32, each = torch.float32, (B,)
+    for t, dt in ((uniforms, f32), (temperature, f32), (top_k, torch.int32), (top_p, f32),
+                  (min_p, f32), (out, torch.int64), (logprobs, f32)):
+        if t is not None and (t.dtype is not dt or t.shape != each or not t.is_contiguous()):
+            _refuse(what, "uniforms, temperature, top_p, min_p and logprobs must be contiguous fp32 "
+                          "[B], top_k int32 [B], out int64 [B]")
+    rc = _call(idx, (_lib or lib()).helm_sample_tokens, logits.data_ptr(), ls[0],
+               helm_dtype(logits.dtype), uniforms.data_ptr(), _ptr(temperature), _ptr(top_k),
+               _ptr(top_p), _ptr(min_p), out.data_ptr(), _ptr(logprobs), B, V,
+               _stream_of(idx, stream))
+    if rc:
+        _check(rc, "helm_sample_tokens")
     return out

@@ -16,8 +16,10 @@
 // sums of up to 2^18 of those fit 64 bits exactly.  Two runs, grids or cluster
 // sizes give the same token.
 //
-// A row is held by one cluster, its logits in the CTAs' shared memory: HBM is
-// read once.  A filter needs its last kept candidate.  A histogram of counts
+// With few rows a row is held by one cluster, its logits in the CTAs' shared
+// memory.  With at least as many rows as SMs one CTA does a row, reading it from
+// L2 once per pass: no cluster barriers, and two rows share an SM, one computing
+// while the other waits (256 x 151936: 197 -> @BIG@ us).  A filter needs its last kept candidate.  A histogram of counts
 // over 2048 equal steps of the logit (equal steps spread a bell-shaped row over
 // the bins; digits of its bit pattern would not) says in which bin it falls:
 // exactly for top-k, and for top-p by an estimate from counts times the weight at
@@ -27,6 +29,9 @@
 //   many: one pass in fp64 sums the weights above the window, per warp, and each
 //        bin's of the window; only the candidates of the bin that the sums point
 //        to are sorted.  The sums serve the draw as well.
+// For a small k the histogram need not see every logit: the threads' own largest
+// ones bound the k-th from below (k of them at or above a bin are k candidates),
+// and the candidates from that bin up are few.
 // Whatever neither can decide (more than 1024 equal logits at the cut, say) is
 // bisected over the order of candidates, pass by pass.
 #include <cooperative_groups.h>
@@ -161,12 +166,12 @@ struct __align__(16) SampleShared {
 
 static_assert(offsetof(SampleShared, hist) % 16 == 0, "");
 
-template <typename T>
+template <typename T, bool kResident>
 struct Sampler {
   static constexpr int kVec = 16 / sizeof(T);
   const SampleArgs& a;
   SampleShared& s;
-  T* slice;
+  const T* slice;    // in shared memory, or the row itself
   cg::cluster_group cluster;
   int base, n;       // first index and number of logits of this CTA
   int vecs;          // 16-byte groups of its slice (padded with -inf)
@@ -176,7 +181,7 @@ struct Sampler {
   float bin_scale;
   float least_logit;  // below it weights round to 0
 
-  __device__ Sampler(const SampleArgs& a_, SampleShared& s_, T* sl)
+  __device__ Sampler(const SampleArgs& a_, SampleShared& s_, const T* sl)
       : a(a_), s(s_), slice(sl), cluster(cg::this_cluster()) {
     lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
@@ -191,20 +196,24 @@ struct Sampler {
   __device__ __forceinline__ int bin(float f) const {
     return max(0, min(kSampBins - 1, static_cast<int>((top - f) * bin_scale)));
   }
-  __device__ __forceinline__ void get(int vec, float (&f)[kVec]) const {
-    const uint4 raw = reinterpret_cast<const uint4*>(slice)[vec];
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = to_float<T>(e[i]);
+  __device__ __forceinline__ uint4 raw(int vec) const {
+    const uint4* p = reinterpret_cast<const uint4*>(slice) + vec;
+    return kResident ? *p : __ldg(p);
   }
   // fn(value, index within the slice) for every logit of vectors v0, v0 + step ..
   template <typename Fn>
   __device__ __forceinline__ void each(int v0, int v1, int step, Fn fn) const {
+    if (v0 >= v1) return;
+    uint4 next = raw(v0);
     for (int v = v0; v < v1; v += step) {
-      float f[kVec];
-      get(v, f);
+      const uint4 now = next;
+      if (v + step < v1) next = raw(v + step);
+      const T* e = reinterpret_cast<const T*>(&now);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) fn(f[i], v * kVec + i);
+      for (int i = 0; i < kVec; ++i) {
+        const float f = to_float<T>(e[i]);
+        fn(kResident || f == f ? f : -INFINITY, v * kVec + i);
+      }
     }
   }
   // A warp owns a contiguous run of vectors, its lanes take turns.
@@ -284,18 +293,10 @@ struct Sampler {
     __syncthreads();
   }
 
-  // Sends the candidates that `pick` selects to the list of rank 0 (counted
-  // before: they fit), which afterwards holds them in no particular order.
-  template <typename Pick>
-  __device__ void gather(Pick pick) {
-    SampleShared* home = cluster.map_shared_rank(&s, 0);
-    each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
-      if (f > -INFINITY && pick(f)) {
-        const uint32_t at = atomicAdd(&home->list_n, 1u);
-        if (at < kSampList) home->list[at] = order_of(f, base + i);
-      }
-    });
-    cluster.sync();
+  // Adds a candidate to rank 0's list (counted beyond its end as well).
+  __device__ __forceinline__ void push(SampleShared* home, float f, int i) const {
+    const uint32_t at = atomicAdd(&home->list_n, 1u);
+    if (at < kSampList) home->list[at] = order_of(f, base + i);
   }
 
   // Rank 0: sorts its list, weighs it and leaves exclusive running sums in
@@ -351,25 +352,53 @@ struct Sampler {
 
   // Cluster-wide histogram of the candidates' logits, and the bins in which the
   // filters' last candidates fall (the last bin where a filter keeps everything).
-  __device__ void histogram(int k, bool use_k, float p, bool use_p) {
-    each(threadIdx.x, vecs, kSampThreads, [&](float f, int) {
-      if (f > -INFINITY) atomicAdd(&s.hist[bin(f)], 1u);
-    });
-    cluster.sync();
-    constexpr int kPer = kSampBins / kSampThreads;
-    static_assert(kPer == 4, "");
-    const int b0 = threadIdx.x * kPer;
-    uint32_t c[kPer] = {0};
+  static constexpr int kPer = kSampBins / kSampThreads;
+  static_assert(kPer == 4, "");
+  // This thread's kPer bins over the whole cluster.
+  __device__ __forceinline__ void cluster_bins(uint32_t (&c)[kPer]) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c[i] = 0;
 #pragma unroll
     for (int r = 0; r < kSampMaxCluster; ++r) {
       if (r < ranks) {
-        const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s, r)->hist + b0);
+        const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s, r)->hist +
+                                                        threadIdx.x * kPer);
         c[0] += x.x;
         c[1] += x.y;
         c[2] += x.z;
         c[3] += x.w;
       }
     }
+  }
+
+  // From the threads' largest logits: a bin at or above which k candidates lie,
+  // the last bin if there is none.
+  __device__ int bound_k(float largest, int k) {
+    if (largest > -INFINITY) atomicAdd(&s.hist[bin(largest)], 1u);
+    if (threadIdx.x == 0) s.bin_k = kSampBins - 1;
+    cluster.sync();
+    uint32_t c[kPer], total;
+    cluster_bins(c);
+    const uint32_t uk = static_cast<uint32_t>(k);
+    uint32_t before = block_scan(c[0] + c[1] + c[2] + c[3],
+                                 reinterpret_cast<uint32_t*>(s.warp_a), total);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (before < uk && before + c[i] >= uk) s.bin_k = threadIdx.x * kPer + i;
+      before += c[i];
+    }
+    __syncthreads();
+    return s.bin_k;
+  }
+
+  __device__ void histogram(int k, bool use_k, float p, bool use_p) {
+    each(threadIdx.x, vecs, kSampThreads, [&](float f, int) {
+      if (f > -INFINITY) atomicAdd(&s.hist[bin(f)], 1u);
+    });
+    cluster.sync();
+    const int b0 = threadIdx.x * kPer;
+    uint32_t c[kPer];
+    cluster_bins(c);
     if (threadIdx.x == 0) {
       s.bin_k = s.bin_p = kSampBins - 1;
       s.in_k = s.upto_k = 0xffffffffu;
@@ -533,6 +562,7 @@ struct Sampler {
   }
 
   __device__ void run(int row, float mx, float mn) {
+    const float own_max = mx;  // this thread's largest logit
     const float temp = a.temperature != nullptr ? a.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
     const int k = greedy || a.top_k == nullptr ? 0 : a.top_k[row];
@@ -587,27 +617,47 @@ struct Sampler {
     const double least = static_cast<double>(mp) * 17592186044416.0;  // min_p in units of 2^-44
 
     // ---- where the filters cut -------------------------------------------------
-    bool few = false;
-    if (use_k || use_p) {
-      histogram(k, use_k, p, use_p);
-      few = (use_k ? s.upto_k : s.upto_w) <= kSampList;
-    }
-
-    // ---- weights of the row -----------------------------------------------------
     const int s0 = seg_begin(warp), s1 = seg_begin(warp + 1);
     u64 row_total = 0, above = 0;
-    if (few) {
-      // Rank 0 finishes the row.  It needs the row's sum for top-p alone and for
-      // the log probability.
+    SampleShared* home = cluster.map_shared_rank(&s, 0);
+    // Sends the candidates of bins 0 .. upto to rank 0, which finishes the row if
+    // they fit its list; sums the row where rank 0 needs that: for top-p without
+    // top-k and for log probabilities.
+    auto try_few = [&](int upto) {
       if (a.logprobs != nullptr || !use_k) {
-        each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight(f); });
-        cluster_sum(row_total, above);
+        each(s0 + lane, s1, 32, [&](float f, int i) {
+          row_total += weight(f);
+          if (f > -INFINITY && bin(f) <= upto) push(home, f, i);
+        });
+      } else {
+        each(s0 + lane, s1, 32, [&](float f, int i) {
+          if (f > -INFINITY && bin(f) <= upto) push(home, f, i);
+        });
       }
-      const int upto = use_k ? s.bin_k : window_begin() + kSampWindow - 1;
-      gather([&](float f) { return bin(f) <= upto; });
+      cluster_sum(row_total, above);
+      if (home->list_n > kSampList) {
+        row_total = above = 0;
+        return false;
+      }
+      cluster.sync();  // all have seen the count: rank 0 may use its list, the others leave
       if (rank == 0) finish_few(row, k, use_k, p, use_p, least, u32, row_total);
-      return;  // rank 0 touches no other CTA's memory from here on
+      return true;  // rank 0 touches no other CTA's memory from here on
+    };
+    if (use_k && k <= ranks * (kSampThreads / 4)) {
+      if (try_few(bound_k(own_max, k))) return;
+      cluster.sync();  // more than the list holds: start over with all logits
+      for (int i = threadIdx.x; i < kSampBins; i += kSampThreads) s.hist[i] = 0;
+      if (threadIdx.x == 0) s.list_n = 0;
+      cluster.sync();
     }
+    if (use_k || use_p) {
+      histogram(k, use_k, p, use_p);
+      if ((use_k ? s.upto_k : s.upto_w) <= kSampList &&
+          try_few(use_k ? s.bin_k : window_begin() + kSampWindow - 1))
+        return;
+    }
+
+    // ---- many candidates, or no filter ------------------------------------------
     u64 last = 0;        // every candidate from this order on is kept
     u64 warp_kept = 0;   // of this warp's run of vectors
     bool known = true;   // warp_kept is right
@@ -827,7 +877,11 @@ struct Sampler {
   __device__ u64 bin_last(int which, bool by_mass, u64 need, u64 above, u64& mass) {
     if (rank == 0 && threadIdx.x == 0) s.list_n = 0;
     cluster.sync();
-    gather([&](float f) { return bin(f) == which; });
+    SampleShared* home = cluster.map_shared_rank(&s, 0);
+    each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
+      if (f > -INFINITY && bin(f) == which) push(home, f, i);
+    });
+    cluster.sync();
     if (rank == 0) {
       const int count = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kSampList)));
       u64 w[2], ex[2], sum;
@@ -853,73 +907,78 @@ struct Sampler {
   }
 };
 
-template <typename T>
+template <typename T, bool kResident>
 __global__ void __launch_bounds__(kSampThreads, 2) sample_tokens_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(s_raw);
   T* slice = reinterpret_cast<T*>(s_raw + (sizeof(SampleShared) + 15) / 16 * 16);
-  Sampler<T> job(a, s, slice);
-  constexpr int kVec = Sampler<T>::kVec;
+  Sampler<T, kResident> job(a, s, slice);
+  constexpr int kVec = 16 / sizeof(T);
   const int row = blockIdx.x / job.ranks;
   job.base = min(a.vocab, job.rank * a.slice);
   job.n = min(a.slice, a.vocab - job.base);
   job.vecs = (job.n + kVec - 1) / kVec;
   const T* src = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.row_stride + job.base;
-  // into shared memory, NaN as -inf and the last vector padded with it
   float mx = -INFINITY, mn = INFINITY;
-  const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  if (kResident) {
+    // into shared memory, NaN as -inf and the last vector padded with it
+    const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll 4
-  for (int v = threadIdx.x; v < job.vecs; v += kSampThreads) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-    if (aligned && (v + 1) * kVec <= job.n) {
-      raw = __ldg(reinterpret_cast<const uint4*>(src) + v);
-    } else {
+    for (int v = threadIdx.x; v < job.vecs; v += kSampThreads) {
+      uint4 raw;
+      T* e = reinterpret_cast<T*>(&raw);
+      if (aligned && (v + 1) * kVec <= job.n) {
+        raw = __ldg(reinterpret_cast<const uint4*>(src) + v);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        e[i] = v * kVec + i < job.n ? src[v * kVec + i] : from_float<T>(-INFINITY);
-    }
+        for (int i = 0; i < kVec; ++i)
+          e[i] = v * kVec + i < job.n ? src[v * kVec + i] : from_float<T>(-INFINITY);
+      }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const float f = to_float<T>(e[i]);
-      if (f != f) e[i] = from_float<T>(-INFINITY);
-      mx = fmaxf(mx, f);  // NaN loses
-      if (f > -INFINITY) mn = fminf(mn, f);
+      for (int i = 0; i < kVec; ++i) {
+        const float f = to_float<T>(e[i]);
+        if (f != f) e[i] = from_float<T>(-INFINITY);
+        mx = fmaxf(mx, f);  // NaN loses
+        if (f > -INFINITY) mn = fminf(mn, f);
+      }
+      reinterpret_cast<uint4*>(slice)[v] = raw;
     }
-    reinterpret_cast<uint4*>(slice)[v] = raw;
+  } else {
+    job.slice = src;  // 16-byte aligned, a whole number of vectors
+#pragma unroll 4
+    for (int v = threadIdx.x; v < job.vecs; v += kSampThreads) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + v);
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const float f = to_float<T>(e[i]);
+        mx = fmaxf(mx, f);
+        if (f > -INFINITY) mn = fminf(mn, f);
+      }
+    }
   }
   job.run(row, mx, mn);
 }
 
-template <typename T>
-cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
+template <typename T, bool kResident>
+cudaError_t launch_sample(SampleArgs a, int batch, int ctas, cudaStream_t stream) {
   static unsigned long long configured = 0;  // one bit per device
+  constexpr int kFixed = (sizeof(SampleShared) + 15) / 16 * 16;
+  static_assert(kFixed + kSampSliceBytes <= 227 * 1024, "");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  constexpr int kFixed = (sizeof(SampleShared) + 15) / 16 * 16;
-  static_assert(kFixed + kSampSliceBytes <= 227 * 1024, "");
-  if (dev >= 64 || !(configured & (1ull << dev))) {
-    e = cudaFuncSetAttribute(sample_tokens_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kFixed + kSampSliceBytes);
+  if (kResident && (dev >= 64 || !(configured & (1ull << dev)))) {
+    e = cudaFuncSetAttribute(sample_tokens_kernel<T, kResident>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kSampSliceBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) configured |= 1ull << dev;
   }
-  // CTAs of a row: as many as hold its logits two to an SM (one to an SM where a
-  // cluster of eight leaves more); more while SMs would be idle and every CTA
-  // keeps a few thousand logits
-  int ctas = 1;
-  auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
-  while (ctas < kSampMaxCluster && static_cast<int64_t>(slice_of(ctas)) * sizeof(T) > kSampSliceGoal)
-    ctas *= 2;
-  while (ctas < kSampMaxCluster && batch * ctas * 2 <= num_sms_current_device() &&
-         slice_of(ctas) > 8192)
-    ctas *= 2;
-  a.slice = slice_of(ctas);
+  a.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));
   cfg.blockDim = dim3(kSampThreads);
-  cfg.dynamicSmemBytes = kFixed + static_cast<size_t>(a.slice) * sizeof(T);
+  cfg.dynamicSmemBytes = kFixed + (kResident ? static_cast<size_t>(a.slice) * sizeof(T) : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -928,7 +987,26 @@ cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, kResident>, a);
+}
+
+template <typename T>
+cudaError_t dispatch_sample(const SampleArgs& a, int batch, cudaStream_t stream) {
+  const int sms = num_sms_current_device();
+  constexpr int kVec = 16 / sizeof(T);
+  if (batch >= sms && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
+      a.row_stride % kVec == 0 && a.vocab % kVec == 0)
+    return launch_sample<T, false>(a, batch, 1, stream);
+  // CTAs of a row: as many as hold its logits two to an SM (one to an SM where a
+  // cluster of eight leaves more); more while SMs would be idle and every CTA
+  // keeps a few thousand logits
+  int ctas = 1;
+  auto bytes = [&](int c) { return (static_cast<int64_t>(a.vocab) + c - 1) / c * static_cast<int64_t>(sizeof(T)); };
+  while (ctas < kSampMaxCluster && bytes(ctas) > kSampSliceGoal) ctas *= 2;
+  while (ctas < kSampMaxCluster && batch * ctas * 2 <= sms &&
+         bytes(ctas) > 8192 * static_cast<int64_t>(sizeof(T)))
+    ctas *= 2;
+  return launch_sample<T, true>(a, batch, ctas, stream);
 }
 
 }  // namespace
@@ -950,13 +1028,13 @@ extern "C" int helm_sample_tokens(const void* logits, int64_t row_stride, int dt
   cudaError_t e;
   switch (dtype) {
     case HELM_DTYPE_BF16:
-      e = launch_sample<__nv_bfloat16>(a, batch, s);
+      e = dispatch_sample<__nv_bfloat16>(a, batch, s);
       break;
     case HELM_DTYPE_FP16:
-      e = launch_sample<__half>(a, batch, s);
+      e = dispatch_sample<__half>(a, batch, s);
       break;
     case HELM_DTYPE_FP32:
-      e = launch_sample<float>(a, batch, s);
+      e = dispatch_sample<float>(a, batch, s);
       break;
     default:
       return HELM_ERR_UNSUPPORTED;
