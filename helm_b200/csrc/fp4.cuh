@@ -41,8 +41,7 @@ struct Fp4Tile {
   }
   // byte offset of K code byte i of token t
   __device__ __forceinline__ static int k_code(int t, int i) {
-    const int chunk = D == 256 ? ((i >> 4) ^ (4 * (t & 1))) : (i >> 4);
-    return row_of(t) * kRow + chunk * 16 + (i & 15);
+    return row_of(t) * kRow + (D == 256 ? i ^ (64 * (t & 1)) : i);
   }
   // XOR applied to a V chunk index of token t
   __device__ __forceinline__ static int v_turn(int t) {

@@ -13,14 +13,9 @@ namespace helm {
 namespace {
 
 struct AppendFp4Args {
-  const void* q;
-  int64_t q_st, q_sh;
-  const void* k;
-  int64_t k_st, k_sh;
-  const void* v;
-  int64_t v_st, v_sh;
-  const void* qw;
-  const void* kw;
+  const void* src[3];     // q, k, v: indexed by a row's kind
+  int64_t st[3], sh[3];   // their token and head strides
+  const void* weight[3];  // norm weights of q and k
   float eps;
   const void* cos;
   const void* sin;
@@ -30,14 +25,13 @@ struct AppendFp4Args {
   uint8_t* pool;
   int64_t pool_rows;  // pool_pages * page_size
   const int64_t* slot_rows;
-  int64_t num_rows;   // tokens * (hq + 2 hkv)
   int hq, hkv, page_size;
-  float k_inv, v_inv;  // 1 / cache scale (a power of two)
+  int page_shift;  // page_size = 1 << page_shift, or -1
+  float inv[3];    // 1 / cache scale (a power of two) of k and v
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void widen8(const uint4& r, float (&x)[8]) {
   const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
@@ -45,16 +39,19 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  uint4 r;
-  T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_float<T>(x[i]);
-  *reinterpret_cast<uint4*>(p) = r;
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(MmaOp<T>::pack(x[0], x[1]), MmaOp<T>::pack(x[2], x[3]),
+                 MmaOp<T>::pack(x[4], x[5]), MmaOp<T>::pack(x[6], x[7]));
 }
 
-// Slot and row inside the page of a pool row (32-bit division where it fits).
-__device__ __forceinline__ void split_row(int64_t row, int page_size, int64_t& slot, int& r_in) {
-  if (row < (int64_t(1) << 32)) {
+// Slot and row inside the page of a pool row (a shift or a 32-bit division where
+// that does).
+__device__ __forceinline__ void split_row(int64_t row, int page_size, int page_shift, int64_t& slot,
+                                          int& r_in) {
+  if (page_shift >= 0) {
+    slot = row >> page_shift;
+    r_in = static_cast<int>(row) & (page_size - 1);
+  } else if (row < (int64_t(1) << 32)) {
     const uint32_t u = static_cast<uint32_t>(row), s = u / static_cast<uint32_t>(page_size);
     slot = s;
     r_in = static_cast<int>(u - s * page_size);
@@ -62,6 +59,28 @@ __device__ __forceinline__ void split_row(int64_t row, int page_size, int64_t& s
     slot = row / page_size;
     r_in = static_cast<int>(row - slot * page_size);
   }
+}
+
+// log2 of a power of two, else -1.
+inline int shift_of(int x) {
+  int s = -1;
+  if ((x & (x - 1)) == 0)
+    while ((1 << ++s) < x) {
+    }
+  return s;
+}
+
+// max that keeps NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // First byte of the tile that holds pool row (slot, r_in) of KV head h.
@@ -72,104 +91,131 @@ __device__ __forceinline__ int64_t tile_base(int64_t slot, int r_in, int h, int 
          Fp4Tile<D>::kBytes;
 }
 
-// One head row of D values on D / 8 lanes, eight values a lane (16-byte loads).
-// A quantisation block is two neighbouring lanes.  Rows of different kinds (q,
-// k, v) may share a warp, so the shuffles run for every lane and the results
-// are selected.  HBM bound: per token 2 (2 Hq + 2 Hkv) D + 1.125 Hkv D bytes.
+// One head row of D values on D / 8 lanes, eight values a lane (16-byte loads);
+// the rows of a warp are neighbouring head rows of one token, so the row's place
+// in the pool is found once per warp and needs no division by the head count.  A
+// quantisation block is two neighbouring lanes.  Rows of different kinds (q, k,
+// v) may share a warp, so the shuffles run for every lane and the results are
+// selected; a warp of q rows alone ends before the quantising half.  Bytes per
+// token: 2 (2 Hq + 2 Hkv) D + 1.125 Hkv D, but at D = 128 the instructions weigh
+// as much (a division per row and quantised q rows cost 41 us where this takes
+// 27: 4096 tokens, 32/8 heads, norm and rotation).
+constexpr int kFp4RowWarps = 8;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_append_fp4_kernel(const AppendFp4Args a) {
+__global__ void __launch_bounds__(kFp4RowWarps * 32) kv_append_fp4_kernel(const AppendFp4Args a) {
   // programmatic dependent launch both ways, as kv_append_kernel
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kLanes = D / 8;
-  const int64_t idx = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  const int part = threadIdx.x % kLanes;  // dims [8 part, 8 part + 8)
-  const bool live = idx < a.num_rows;
-  const int per_tok = a.hq + 2 * a.hkv;
-  const int64_t tok = live ? idx / per_tok : 0;
-  const int hr = live ? static_cast<int>(idx - tok * per_tok) : 0;
-  const bool is_q = hr < a.hq, is_v = hr >= a.hq + a.hkv;
-  const int h = is_q ? hr : (is_v ? hr - a.hq - a.hkv : hr - a.hq);
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t tok = blockIdx.x;
+  const int part = lane % kLanes;  // dims [8 part, 8 part + 8)
+  const int want = (blockIdx.y * kFp4RowWarps + warp) * kRows + lane / kLanes;
+  const int rows = a.hq + 2 * a.hkv;
+  if ((blockIdx.y * kFp4RowWarps + warp) * kRows >= rows) return;  // the whole warp
+  const bool live = want < rows;
+  const int hr = live ? want : rows - 1;
+  const int kind = hr < a.hq ? 0 : (hr < a.hq + a.hkv ? 1 : 2);
+  const bool is_q = kind == 0, is_v = kind == 2;
+  const int h = hr - (is_q ? 0 : (is_v ? a.hq + a.hkv : a.hq));
+  // everything the row needs is loaded at once
+  const T* w = static_cast<const T*>(a.weight[kind]);
+  const bool turn = a.cos != nullptr && !is_v;
+  uint4 raw_w = {}, raw_c = {}, raw_s = {};
+  const uint4 raw_x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.src[kind]) +
+                                                      tok * a.st[kind] + h * a.sh[kind] + part * 8);
+  if (w != nullptr) raw_w = *reinterpret_cast<const uint4*>(w + part * 8);
+  if (turn) {
+    raw_c = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.cos) + tok * a.rope_st + part * 8);
+    raw_s = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.sin) + tok * a.rope_st + part * 8);
+  }
+  const int64_t row = is_q ? -1 : a.slot_rows[tok];
   float x[8];
-  const T* src = is_q ? static_cast<const T*>(a.q) + tok * a.q_st + h * a.q_sh
-                      : (is_v ? static_cast<const T*>(a.v) + tok * a.v_st + h * a.v_sh
-                              : static_cast<const T*>(a.k) + tok * a.k_st + h * a.k_sh);
-  load8<T>(src + part * 8, x);
-  const T* w = static_cast<const T*>(is_q ? a.qw : (is_v ? nullptr : a.kw));
-  if (a.qw != nullptr || a.kw != nullptr) {
+  widen8<T>(raw_x, x);
+  if (__any_sync(0xffffffffu, w != nullptr)) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
     ss = warp_sum_xor(ss, 1, kLanes / 2);
     if (w != nullptr) {
-      const float r = 1.f / sqrtf(ss / static_cast<float>(D) + a.eps);
+      const float r = rsqrtf(fmaf(ss, 1.f / static_cast<float>(D), a.eps));
       float wv[8];
-      load8<T>(w + part * 8, wv);
+      widen8<T>(raw_w, wv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wv[i];
     }
   }
-  if (a.cos != nullptr) {
+  if (__any_sync(0xffffffffu, turn)) {
     float other[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
-    if (!is_v) {
+    if (turn) {
       float c[8], s[8];
-      load8<T>(static_cast<const T*>(a.cos) + tok * a.rope_st + part * 8, c);
-      load8<T>(static_cast<const T*>(a.sin) + tok * a.rope_st + part * 8, s);
-      const float sign = part < kLanes / 2 ? -1.f : 1.f;
+      widen8<T>(raw_c, c);
+      // rotate_half negates the partner of the lower half: the sine's sign does
+      const uint32_t flip = part < kLanes / 2 ? 0x80008000u : 0u;
+      raw_s.x ^= flip;
+      raw_s.y ^= flip;
+      raw_s.z ^= flip;
+      raw_s.w ^= flip;
+      widen8<T>(raw_s, s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + sign * other[i] * s[i];
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(other[i], s[i], x[i] * c[i]);
     }
   }
-  if (is_q) {
-    if (live) store8<T>(static_cast<T*>(a.q_out) + tok * a.qo_st + h * a.qo_sh + part * 8, x);
-  }
-  // ---- quantise (q rows take part in the shuffles only) ----------------------
-  const float inv_cache = is_v ? a.v_inv : a.k_inv;
+  if (is_q && live) store8<T>(static_cast<T*>(a.q_out) + tok * a.qo_st + h * a.qo_sh + part * 8, x);
+  if (__all_sync(0xffffffffu, is_q)) return;
+  // ---- quantise (q rows take part in the shuffle only) -----------------------
+  const float inv_cache = a.inv[kind];
   float amax = 0.f;
-  bool nan = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     x[i] *= inv_cache;
-    nan |= x[i] != x[i];
-    amax = fmaxf(amax, fabsf(x[i]));
+    amax = max_nan(amax, fabsf(x[i]));
   }
-  if (nan) amax = NAN;  // a NaN marks its whole block
-  const float peer = __shfl_xor_sync(0xffffffffu, amax, 1);
-  nan = amax != amax || peer != peer;
-  amax = fmaxf(amax, peer);
-  if (!live || is_q) return;
-  const int64_t row = a.slot_rows[tok];
-  if (row < 0) return;
+  amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));  // NaN marks the whole block
+  if (!live || row < 0) return;
   if (row >= a.pool_rows) {
     if (part == 0) report_status(HELM_DEV_BAD_PAGE);
     return;
   }
-  const uint32_t s8 = nan ? 0x7fu : float_to_e4m3(amax / 6.f);
+  // max / 6 rounded to nearest: one step of refinement on the rounded product
+  const float sixth = amax * (1.f / 6.f);
+  const float most = amax < INFINITY ? fmaf(fmaf(-6.f, sixth, amax), 1.f / 6.f, sixth) : amax;
+  const uint32_t s8 = amax != amax ? 0x7fu : float_to_e4m3(most);
   const uint32_t sh = e4m3x2_to_half2(s8);
   const float s = __low2float(*reinterpret_cast<const __half2*>(&sh));
-  // x / s correctly rounded: one Newton step on the product with the rounded
-  // reciprocal (s has four significant bits), so a value on the border between
-  // two codes is seen on the border
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  // x / s, refined likewise.  s has four significant bits and the borders between
+  // codes three, so a border is met exactly, and the value next to it is at least
+  // 1.06 half steps of the quotient away: it stays on its side.
+  const float r0 = rcp_fast(s);
+  const float inv = s > 0.f ? fmaf(fmaf(-s, r0, 1.f), r0, r0) : 0.f;
+  if (!(amax < INFINITY)) {  // infinities saturate
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -3.0e38f), 3.0e38f);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf(x[i], -3.0e38f), 3.0e38f);  // infinities saturate
-    const float q0 = y * inv;
-    x[i] = copysignf(fmaf(fmaf(-q0, s, y), inv, q0), y);  // -0 stays -0
+    const float q0 = x[i] * inv;
+    x[i] = fmaf(-fmaf(q0, s, -x[i]), inv, q0);  // (this way round, -0 stays -0)
   }
   const uint32_t codes = float8_to_fp4(x);
   int64_t slot;
   int r_in;
-  split_row(row, a.page_size, slot, r_in);
+  split_row(row, a.page_size, a.page_shift, slot, r_in);
   const int t = r_in & (kFp4TileTokens - 1);
   uint8_t* tile = a.pool + tile_base<D>(slot, r_in, h, a.hkv, a.page_size);
   using L = Fp4Tile<D>;
-  *reinterpret_cast<uint32_t*>(tile + (is_v ? L::v_code(t, part * 4) : L::k_code(t, part * 4))) =
-      codes;
-  if ((part & 1) == 0)
-    tile[is_v ? L::v_scale(t, part >> 1) : L::k_scale(t, part >> 1)] = static_cast<uint8_t>(s8);
+  // (a branch: the rows of a warp are mostly of one kind, and each side's
+  // offsets are a dozen instructions)
+  if (is_v) {
+    *reinterpret_cast<uint32_t*>(tile + L::v_code(t, part * 4)) = codes;
+    if ((part & 1) == 0) tile[L::v_scale(t, part >> 1)] = static_cast<uint8_t>(s8);
+  } else {
+    *reinterpret_cast<uint32_t*>(tile + L::k_code(t, part * 4)) = codes;
+    if ((part & 1) == 0) tile[L::k_scale(t, part >> 1)] = static_cast<uint8_t>(s8);
+  }
 }
 
 struct GatherFp4Args {
@@ -180,19 +226,18 @@ struct GatherFp4Args {
   int64_t ko_st, ko_sh;
   void* v_out;
   int64_t vo_st, vo_sh;
-  int64_t num_rows;  // tokens * 2 hkv
-  int hkv, page_size;
+  int hkv, page_size, page_shift;
   float k_scale, v_scale;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) gather_rows_fp4_kernel(const GatherFp4Args a) {
-  constexpr int kLanes = D / 8;
-  const int64_t idx = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  const int part = threadIdx.x % kLanes;
-  if (idx >= a.num_rows) return;
-  const int64_t tok = idx / (2 * a.hkv);
-  const int hr = static_cast<int>(idx - tok * (2 * a.hkv));
+__global__ void __launch_bounds__(kFp4RowWarps * 32) gather_rows_fp4_kernel(const GatherFp4Args a) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t tok = blockIdx.x;
+  const int part = lane % kLanes;
+  const int hr = (blockIdx.y * kFp4RowWarps + warp) * kRows + lane / kLanes;
+  if (hr >= 2 * a.hkv) return;
   const bool is_v = hr >= a.hkv;
   const int h = is_v ? hr - a.hkv : hr;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -202,13 +247,18 @@ __global__ void __launch_bounds__(256) gather_rows_fp4_kernel(const GatherFp4Arg
   } else if (row >= 0) {
     int64_t slot;
     int r_in;
-    split_row(row, a.page_size, slot, r_in);
+    split_row(row, a.page_size, a.page_shift, slot, r_in);
     const int t = r_in & (kFp4TileTokens - 1);
     const uint8_t* tile = a.pool + tile_base<D>(slot, r_in, h, a.hkv, a.page_size);
     using L = Fp4Tile<D>;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(
-        tile + (is_v ? L::v_code(t, part * 4) : L::k_code(t, part * 4)));
-    const uint32_t s8 = tile[is_v ? L::v_scale(t, part >> 1) : L::k_scale(t, part >> 1)];
+    uint32_t codes, s8;
+    if (is_v) {
+      codes = *reinterpret_cast<const uint32_t*>(tile + L::v_code(t, part * 4));
+      s8 = tile[L::v_scale(t, part >> 1)];
+    } else {
+      codes = *reinterpret_cast<const uint32_t*>(tile + L::k_code(t, part * 4));
+      s8 = tile[L::k_scale(t, part >> 1)];
+    }
     const uint32_t sh = e4m3x2_to_half2(s8);
     const float s = __low2float(*reinterpret_cast<const __half2*>(&sh)) *
                     (is_v ? a.v_scale : a.k_scale);
@@ -235,12 +285,17 @@ bool rows16_misaligned(const void* p, std::initializer_list<int64_t> strides) {
   return false;
 }
 
+// One block of kFp4RowWarps warps per token and run of head rows.
+dim3 fp4_row_grid(int tokens, int rows, int head_dim) {
+  const int per_block = kFp4RowWarps * 32 / (head_dim / 8);
+  return dim3(static_cast<unsigned>(tokens), static_cast<unsigned>((rows + per_block - 1) / per_block));
+}
+
 template <typename T>
-cudaError_t launch_append_fp4(int head_dim, const AppendFp4Args& a, cudaStream_t s) {
+cudaError_t launch_append_fp4(int head_dim, int tokens, const AppendFp4Args& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  const int64_t threads = a.num_rows * (head_dim / 8);
-  cfg.gridDim = dim3(static_cast<unsigned>((threads + 255) / 256));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = fp4_row_grid(tokens, a.hq + 2 * a.hkv, head_dim);
+  cfg.blockDim = dim3(kFp4RowWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -258,18 +313,17 @@ cudaError_t launch_append_fp4(int head_dim, const AppendFp4Args& a, cudaStream_t
 }
 
 template <typename T>
-cudaError_t launch_gather_fp4(int head_dim, const GatherFp4Args& a, cudaStream_t s) {
-  const int64_t threads = a.num_rows * (head_dim / 8);
-  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+cudaError_t launch_gather_fp4(int head_dim, int tokens, const GatherFp4Args& a, cudaStream_t s) {
+  const dim3 grid = fp4_row_grid(tokens, 2 * a.hkv, head_dim), block(kFp4RowWarps * 32);
   switch (head_dim) {
     case 64:
-      gather_rows_fp4_kernel<T, 64><<<grid, 256, 0, s>>>(a);
+      gather_rows_fp4_kernel<T, 64><<<grid, block, 0, s>>>(a);
       break;
     case 128:
-      gather_rows_fp4_kernel<T, 128><<<grid, 256, 0, s>>>(a);
+      gather_rows_fp4_kernel<T, 128><<<grid, block, 0, s>>>(a);
       break;
     default:
-      gather_rows_fp4_kernel<T, 256><<<grid, 256, 0, s>>>(a);
+      gather_rows_fp4_kernel<T, 256><<<grid, block, 0, s>>>(a);
   }
   return cudaGetLastError();
 }
@@ -289,9 +343,9 @@ int fp4_rows_check(const void* pool, int64_t pool_pages, const void* slot_rows, 
   return HELM_OK;
 }
 
-// Threads of a launch must fit a 31-bit grid of 256-thread blocks.
+// The run of head rows is a grid's second dimension.
 bool fp4_grid_fits(int64_t rows, int head_dim) {
-  return rows <= (int64_t(1) << 38) && (rows * (head_dim / 8) + 255) / 256 < (int64_t(1) << 31);
+  return rows < (int64_t(1) << 30) && fp4_row_grid(1, static_cast<int>(rows), head_dim).y <= 65535;
 }
 
 }  // namespace
@@ -331,17 +385,18 @@ extern "C" int helm_kv_append_fp4(const void* q, int64_t q_stride_t, int64_t q_s
     return HELM_ERR_ALIGNMENT;
   if (num_tokens == 0) return HELM_OK;
   AppendFp4Args a;
-  a.q = q;
-  a.q_st = q_stride_t;
-  a.q_sh = q_stride_h;
-  a.k = k;
-  a.k_st = k_stride_t;
-  a.k_sh = k_stride_h;
-  a.v = v;
-  a.v_st = v_stride_t;
-  a.v_sh = v_stride_h;
-  a.qw = q_norm_w;
-  a.kw = k_norm_w;
+  a.src[0] = q;
+  a.st[0] = q_stride_t;
+  a.sh[0] = q_stride_h;
+  a.src[1] = k;
+  a.st[1] = k_stride_t;
+  a.sh[1] = k_stride_h;
+  a.src[2] = v;
+  a.st[2] = v_stride_t;
+  a.sh[2] = v_stride_h;
+  a.weight[0] = q_norm_w;
+  a.weight[1] = k_norm_w;
+  a.weight[2] = nullptr;
   a.eps = eps;
   a.cos = cos;
   a.sin = sin;
@@ -354,14 +409,17 @@ extern "C" int helm_kv_append_fp4(const void* q, int64_t q_stride_t, int64_t q_s
   a.slot_rows = slot_rows;
   a.hq = q != nullptr ? num_q_heads : 0;
   a.hkv = num_kv_heads;
-  a.num_rows = static_cast<int64_t>(num_tokens) * (a.hq + 2 * a.hkv);
   a.page_size = page_size;
-  a.k_inv = 1.f / k_scale;
-  a.v_inv = 1.f / v_scale;
-  if (!fp4_grid_fits(a.num_rows, head_dim)) return HELM_ERR_UNSUPPORTED;
+  a.page_shift = shift_of(page_size);
+  a.inv[0] = 1.f;
+  a.inv[1] = 1.f / k_scale;
+  a.inv[2] = 1.f / v_scale;
+  if (!fp4_grid_fits(static_cast<int64_t>(a.hq) + 2 * static_cast<int64_t>(a.hkv), head_dim))
+    return HELM_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == HELM_DTYPE_BF16 ? launch_append_fp4<__nv_bfloat16>(head_dim, a, s)
-                                                 : launch_append_fp4<__half>(head_dim, a, s);
+  const cudaError_t e = dtype == HELM_DTYPE_BF16
+                            ? launch_append_fp4<__nv_bfloat16>(head_dim, num_tokens, a, s)
+                            : launch_append_fp4<__half>(head_dim, num_tokens, a, s);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return HELM_ERR_CUDA;
@@ -395,15 +453,16 @@ extern "C" int helm_gather_kv_rows_fp4(const void* kv_pool, int64_t pool_pages,
   a.v_out = v_out;
   a.vo_st = v_out_stride_t;
   a.vo_sh = v_out_stride_h;
-  a.num_rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
   a.hkv = num_kv_heads;
   a.page_size = page_size;
+  a.page_shift = shift_of(page_size);
   a.k_scale = k_scale;
   a.v_scale = v_scale;
-  if (!fp4_grid_fits(a.num_rows, head_dim)) return HELM_ERR_UNSUPPORTED;
+  if (!fp4_grid_fits(2 * static_cast<int64_t>(num_kv_heads), head_dim)) return HELM_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == HELM_DTYPE_BF16 ? launch_gather_fp4<__nv_bfloat16>(head_dim, a, s)
-                                                 : launch_gather_fp4<__half>(head_dim, a, s);
+  const cudaError_t e = dtype == HELM_DTYPE_BF16
+                            ? launch_gather_fp4<__nv_bfloat16>(head_dim, num_tokens, a, s)
+                            : launch_gather_fp4<__half>(head_dim, num_tokens, a, s);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return HELM_ERR_CUDA;
