@@ -571,7 +571,7 @@ def _tp_decode(name: str, args, rank: int, world: int, dev: torch.device, steps:
         n_split = getattr(args, "shard_of", 0) or world
         shard = synthetic_shard(arch, rank if n_split == world else 0, n_split, w["dtype"], dev)
         tp = TPDecodeModel(shard, batch=Bq, max_len=ctx + 3 + W + K + e2e_steps + 16,
-                           page_size=16)
+                           page_size=16, kv_format=getattr(args, "kv_format", "model"))
     try:
         tp.fill_kv(ctx)
         for _ in range(3):
@@ -617,6 +617,9 @@ def _tp_decode(name: str, args, rank: int, world: int, dev: torch.device, steps:
             a, b = tp.range
             mean_ctx = (b - a) + ((3 + W + K / 2) if tp.tail else 0)
         kv_bytes = len(shard.layers) * Bq * mean_ctx * 2 * shard.hkv * shard.head_dim * 2
+        fp4 = not seq and tp.fp4
+        if fp4:   # 4.5 bits a value
+            kv_bytes = kv_bytes * 9 / 32
         n_layers = len(shard.layers)
     finally:
         tp.close()
@@ -631,7 +634,8 @@ def _tp_decode(name: str, args, rank: int, world: int, dev: torch.device, steps:
                 hbm=hbm, peak_src=peak_src, n_layers=n_layers,
                 tok_s=Bq / (ms / 1e3), roofline_tok_s=Bq / (step_bytes / (hbm * 1e9)),
                 workload=(f"{name}: {w['name']} random-init, batch {Bq}, {ctx}-token context "
-                          f"(K/V filled synthetically), greedy decode, 16-token pages, " + (
+                          f"(K/V filled synthetically), greedy decode, 16-token pages, "
+                          + ("4-bit K/V, " if fp4 else "") + (
                               f"K/V sequence-split x{world} (token ranges), weights replicated"
                               if seq else
                               f"tensor parallel x{world} (KV heads, q/k/v/gate/up rows, "
@@ -1153,6 +1157,9 @@ def main():
                     help="config4/config5 over N GPUs: tensor parallel with KV heads sharded "
                          "(head), or the whole model on every rank with the K/V split by "
                          "token range and partial states merged over NVLink (sequence)")
+    ap.add_argument("--kv-format", choices=["model", "fp4"], default="model",
+                    help="config4/config5, --kv-split head: K/V in the model dtype, or in 4-bit "
+                         "pages that the device hands out")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--shard-of", type=int, default=0,
                     help="config4/config5 on one GPU: run rank 0's shard of an N-way tensor-"

@@ -16,6 +16,8 @@ from typing import Optional
 
 import torch
 
+from .sampling import SamplingParams, TokenSampler
+
 
 class DecodeLoop:
     def __init__(self, model, kv_offload_mgr=None, dtype: Optional[torch.dtype] = None):
@@ -81,8 +83,10 @@ class DecodeLoop:
 
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens: int = 8, attention_mask=None,
-                 eos_token_id=None, pad_token_id=None, forced_tokens=None, keep_logits=False):
-        """Greedy tokens [B, n].  forced_tokens [B, >= n] (optional) feeds those
+                 eos_token_id=None, pad_token_id=None, forced_tokens=None, keep_logits=False,
+                 sampling: Optional[SamplingParams] = None):
+        """Greedy tokens [B, n], or tokens drawn as `sampling` says (wherever
+        "argmax" stands here).  forced_tokens [B, >= n] (optional) feeds those
         tokens instead of the argmax (teacher forcing) while still returning the
         argmax of every step; keep_logits also returns each step's logits."""
         if self.kv_offload_mgr is not None:
@@ -91,6 +95,7 @@ class DecodeLoop:
         am = torch.ones_like(input_ids) if attention_mask is None else attention_mask.long()
         prompt_lengths = am.sum(dim=1)
         logits = self.prefill(input_ids, am)
+        sampler = None if sampling is None else TokenSampler(sampling, B, logits.device)
         out_tokens, all_logits = [], []
         finished = torch.zeros(B, dtype=torch.bool, device=logits.device)
         terminal = pad_token_id if pad_token_id is not None else eos_token_id
@@ -99,7 +104,11 @@ class DecodeLoop:
         for step in range(max_new_tokens):
             if keep_logits:
                 all_logits.append(logits.float())
-            nxt = torch.argmax(logits, dim=-1, keepdim=True)
+            if sampler is None:
+                nxt = torch.argmax(logits, dim=-1, keepdim=True)
+            else:
+                sampler.tick()
+                nxt = sampler(logits).clone()
             if finished.any() and terminal is not None:
                 nxt = nxt.clone()
                 nxt[finished] = terminal

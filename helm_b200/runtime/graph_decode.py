@@ -32,6 +32,7 @@ import torch
 from .. import _capi
 from .kv_allocator import ARENA_SLOTS
 from .kv_cache import _page_bytes_used, _record_prefetch, _stager_for
+from .sampling import SamplingParams, TokenSampler
 
 
 class _ColdPages:
@@ -195,6 +196,7 @@ class GraphDecoder:
             self.stage = FusedDecodeStage(model, max_batch)
         self.h2d_bytes = 0
         self._steady = None
+        self.sampler: Optional[TokenSampler] = None
 
     # -- host side of a step ------------------------------------------------------
     def _plan(self) -> None:
@@ -341,7 +343,10 @@ class GraphDecoder:
             out = self.model(input_ids=self.ids, attention_mask=ctx.mask4d, position_ids=self.pos,
                              use_cache=False, logits_to_keep=1)
             self.logits.copy_(out.logits[:, -1, :])
-        self.ids.copy_(torch.argmax(self.logits, dim=-1, keepdim=True))
+        if self.sampler is None:
+            self.ids.copy_(torch.argmax(self.logits, dim=-1, keepdim=True))
+        else:
+            self.ids.copy_(self.sampler(self.logits))
         self.pos.add_(1)
         ctx.end_step()
 
@@ -371,8 +376,10 @@ class GraphDecoder:
 
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens: int, keep_logits: bool = False,
-                 reserve_pages: bool = True, forced_tokens=None):
-        """Greedy tokens [B, n] (and, with keep_logits, each step's logits).
+                 reserve_pages: bool = True, forced_tokens=None,
+                 sampling: Optional[SamplingParams] = None):
+        """Greedy tokens [B, n] (and, with keep_logits, each step's logits), or
+        tokens drawn as `sampling` says (wherever "argmax" stands here).
         forced_tokens [B, >= n-1] (teacher forcing): step s+1 is fed
         forced_tokens[:, s] instead of the argmax, which is still returned."""
         from .decode_loop import DecodeLoop
@@ -396,7 +403,12 @@ class GraphDecoder:
         self._steady = None
         self.ctx = _GraphContext(self.mgr, B, self.Hq, self.D, self.L, self.max_len, self.dtype,
                                  self.dev)
-        self.ids = torch.argmax(logits0, dim=-1, keepdim=True)
+        self.sampler = None if sampling is None else TokenSampler(sampling, B, self.dev)
+        if self.sampler is None:
+            self.ids = torch.argmax(logits0, dim=-1, keepdim=True)
+        else:
+            self.sampler.tick()
+            self.ids = self.sampler(logits0).clone()
         self.pos = torch.full((B, 1), S, dtype=torch.long, device=self.dev)
         self.logits = torch.empty_like(logits0)
         history = torch.empty(B, max_new_tokens, dtype=torch.long, device=self.dev)
@@ -416,6 +428,8 @@ class GraphDecoder:
         for step in range(1, max_new_tokens):
             t0 = time.perf_counter()
             self._plan()
+            if self.sampler is not None:
+                self.sampler.tick()
             self.plan_seconds += time.perf_counter() - t0
             if self.graph is None or self._pending_sig != self.cold_sig:
                 if step == 1:

@@ -20,6 +20,12 @@ step.  The decode step is captured as one CUDA graph; lengths, rows, positions
 and the next token advance on the device, so a step needs no host work.  The
 K/V layout is static (dense page tables, all pages resident): the model-level
 multi-GPU form of the decode hot path, without the single-GPU offload policy.
+
+With kv_format "fp4" the cache holds 4.5 bits a value (fp4_pool) and pages are
+handed out by the device: every step starts with helm_build_step_tables, from the
+sequences' lengths and what each does in the step (new_lens: 1 token, idle, or
+leaving).  One page table serves all layers, and sequences of different lengths
+share the pages.
 """
 from __future__ import annotations
 
@@ -30,6 +36,7 @@ import torch
 import torch.distributed as dist
 
 from .. import _capi
+from .sampling import SamplingParams, TokenSampler
 
 
 @dataclass
@@ -169,15 +176,28 @@ class _PeerBuffers:
 
 
 class TPDecodeModel:
-    """Greedy decode of B sequences with this rank's TPWeights.
+    """Greedy decode of B sequences with this rank's TPWeights, or sampled as
+    `sampling` says (every rank draws the same token from the gathered logits).
 
     fill_kv() (synthetic context) or decode steps fed with prompt tokens
     (step(..., forced)) build the cache; step() advances every sequence by one
     token; capture()/replay() run the step as a CUDA graph.
+
+    kv_format "model": K/V in the model dtype, max_len tokens of pages per sequence.
+    "fp4": 4-bit pages, `num_pages` of them per layer for all sequences together
+    (default: max_len tokens each).  set_step() says which sequences take part in
+    the following steps; one that leaves gives its pages back and starts anew at
+    length 0.  A step that runs out of pages records HELM_DEV_NO_PAGES
+    (_capi.device_status) and leaves the sequences concerned as they were.
     """
 
     def __init__(self, w: TPWeights, batch: int, max_len: int, page_size: int = 16,
-                 group: Optional[dist.ProcessGroup] = None):
+                 group: Optional[dist.ProcessGroup] = None, kv_format: str = "model",
+                 num_pages: Optional[int] = None, sampling: Optional[SamplingParams] = None):
+        if kv_format not in ("model", "fp4"):
+            raise ValueError(f"kv_format must be 'model' or 'fp4', not {kv_format!r}")
+        if num_pages is not None and kv_format != "fp4":
+            raise ValueError("num_pages is for kv_format 'fp4'")
         self.w = w
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -191,11 +211,28 @@ class TPDecodeModel:
         self.maxp = -(-max_len // page_size)
         self.max_len = max_len
         dev, L, B = self.dev, self.L, batch
-        # pool[slot][kv][head][token][dim]; layer l, sequence b, page i -> slot (l*B + b)*maxp + i
-        self.pool = torch.empty(L * B * self.maxp, 2, w.hkv, page_size, w.head_dim, dtype=self.dtype,
-                                device=dev)
-        base = torch.arange(L * B, dtype=torch.int32, device=dev).view(L, B, 1) * self.maxp
-        self.tables = (base + torch.arange(self.maxp, dtype=torch.int32, device=dev)).contiguous()
+        self.fp4 = kv_format == "fp4"
+        if self.fp4:
+            pages = B * self.maxp if num_pages is None else num_pages
+            self.pools = [_capi.fp4_pool(pages, w.hkv, page_size, w.head_dim, dev)
+                          for _ in range(L)]
+            i32 = dict(dtype=torch.int32, device=dev)
+            self.table = torch.full((B, self.maxp), -1, **i32)
+            self.free_pages = torch.arange(pages - 1, -1, -1, **i32)   # page 0 goes first
+            self.free_count = torch.tensor([pages], **i32)
+            self.new_lens = torch.ones(B, **i32)
+            self.lens1 = torch.zeros(B, **i32)
+            self._cu = torch.zeros(B + 1, **i32)
+            self._tok = dict(seq_ids=torch.empty(B, **i32), positions=torch.empty(B, **i32),
+                             slot_rows=torch.empty(B, dtype=torch.long, device=dev))
+        else:
+            # pool[slot][kv][head][token][dim]; layer l, sequence b, page i -> slot (l*B + b)*maxp + i
+            self.pool = torch.empty(L * B * self.maxp, 2, w.hkv, page_size, w.head_dim,
+                                    dtype=self.dtype, device=dev)
+            base = torch.arange(L * B, dtype=torch.int32, device=dev).view(L, B, 1) * self.maxp
+            self.tables = (base + torch.arange(self.maxp, dtype=torch.int32,
+                                               device=dev)).contiguous()
+        self.sampler = None if sampling is None else TokenSampler(sampling, B, dev)
         self.lens = torch.zeros(B, dtype=torch.int32, device=dev)      # tokens cached
         self.ids = torch.zeros(B, 1, dtype=torch.long, device=dev)
         self.h = torch.empty(B, self.H, dtype=self.dtype, device=dev)
@@ -221,8 +258,32 @@ class TPDecodeModel:
         if length >= self.max_len:
             raise ValueError("context does not fit max_len")
         g = torch.Generator(device=self.dev).manual_seed(seed * 7919 + self.rank)
-        self.pool.normal_(generator=g)
-        self.lens.fill_(length)
+        if not self.fp4:
+            self.pool.normal_(generator=g)
+            self.lens.fill_(length)
+            return
+        rows = _capi.build_step_tables(
+            self.lens, (length - self.lens).int(), self.table, self.free_pages, self.free_count,
+            page_size=self.P, num_rows=self.B * length, kv_lens=self.lens)[4]
+        if _capi.device_status(self.dev) & _capi.DEV_NO_PAGES:
+            raise ValueError("context does not fit the pages")
+        shape = (min(16384, rows.numel()), self.w.hkv, self.D)
+        for pool in self.pools:
+            k, v = (torch.randn(shape, generator=g, device=self.dev).to(self.dtype) for _ in range(2))
+            for at in range(0, rows.numel(), shape[0]):
+                r = rows[at:at + shape[0]]
+                _capi.kv_append_fp4(k=k[:r.numel()], v=v[:r.numel()], pool=pool, slot_rows=r,
+                                    page_size=self.P)
+
+    @torch.no_grad()
+    def set_step(self, new_lens) -> None:
+        """What the sequences do in the following steps ("fp4" only): per sequence
+        1 (a token), 0 (idle) or -1 (leaves, then idle at length 0)."""
+        if not self.fp4:
+            raise ValueError("set_step needs kv_format 'fp4'")
+        if len(new_lens) != self.B or any(n not in (-1, 0, 1) for n in new_lens):
+            raise ValueError("new_lens: 1, 0 or -1 for each sequence")
+        self.new_lens.copy_(torch.tensor(list(new_lens), dtype=torch.int32))
 
     def close(self) -> None:
         self.graph = None
@@ -249,8 +310,22 @@ class TPDecodeModel:
                 _capi.decode_gemv_allreduce(self.peers.ptrs, self.rank, x[b0:b1], w,
                                             out=out[b0:b1], residual=out[b0:b1])
 
-    @torch.no_grad()
+    def _fp4_rows(self) -> torch.Tensor:
+        """Tables of the step; the pool row of each sequence's token (-1: none)."""
+        _capi.build_step_tables(self.lens, self.new_lens, self.table, self.free_pages,
+                                self.free_count, page_size=self.P, num_rows=self.B,
+                                kv_lens=self.lens1, cu_tokens=self._cu, **self._tok)
+        mine = self._tok["slot_rows"].index_select(0, self._cu[:-1].clamp(max=self.B - 1))
+        return torch.where(self.new_lens > 0, mine, -1)
+
     def step(self, forced: Optional[torch.Tensor] = None) -> None:
+        """_step(), with the host's part of sampling."""
+        if self.sampler is not None:
+            self.sampler.tick()
+        self._step(forced)
+
+    @torch.no_grad()
+    def _step(self, forced: Optional[torch.Tensor] = None) -> None:
         """One decode step: the token in self.ids is appended at position
         lens and attended; self.ids becomes the greedy next token (or, when
         `forced` [B, 1] is given, that token; the argmax stays in self.next)."""
@@ -261,11 +336,15 @@ class TPDecodeModel:
         freqs = pos * self.inv_freq.view(1, -1)
         emb = torch.cat([freqs, freqs], dim=-1)
         cos, sin = emb.cos().to(self.dtype), emb.sin().to(self.dtype)
-        page = (self.lens // P).long()
-        r_in = (self.lens % P).long()
-        slot = self.tables[:, torch.arange(B, device=self.dev), page].long()      # [L, B]
-        rows = (slot * P + r_in.view(1, B)).contiguous()
-        lens1 = self.lens + 1
+        if self.fp4:
+            rows = self._fp4_rows()
+            lens1 = self.lens1
+        else:
+            page = (self.lens // P).long()
+            r_in = (self.lens % P).long()
+            slot = self.tables[:, torch.arange(B, device=self.dev), page].long()      # [L, B]
+            rows = (slot * P + r_in.view(1, B)).contiguous()
+            lens1 = self.lens + 1
         scale = D ** -0.5
         for l, lw in enumerate(w.layers):
             self._gemv(h, lw.wqkv, self.qkv, norm_w=lw.ln1, eps=lw.eps1)
@@ -273,29 +352,45 @@ class TPDecodeModel:
             q = self.qkv[:, :nq].view(B, w.hq, D)
             k = self.qkv[:, nq:nq + nk].view(B, w.hkv, D)
             v = self.qkv[:, nq + nk:].view(B, w.hkv, D)
-            _capi.kv_append(q=q, k=k, v=v, q_out=self.q_out, q_norm_w=lw.q_norm,
-                            k_norm_w=lw.k_norm, eps=lw.qk_eps, cos=cos, sin=sin, pool=self.pool,
-                            slot_rows=rows[l], page_size=P)
-            _capi.paged_decode_attention(self.q_out, self.pool, self.tables[l], lens1,
-                                         num_kv_heads=w.hkv, page_size=P, scale=scale,
-                                         out=self.attn, max_kv_len_hint=self.max_len)
+            if self.fp4:
+                _capi.kv_append_fp4(q=q, k=k, v=v, q_out=self.q_out, q_norm_w=lw.q_norm,
+                                    k_norm_w=lw.k_norm, eps=lw.qk_eps, cos=cos, sin=sin,
+                                    pool=self.pools[l], slot_rows=rows, page_size=P)
+                _capi.paged_decode_attention_fp4(
+                    self.q_out, self.pools[l], self.table, lens1, num_kv_heads=w.hkv, page_size=P,
+                    scale=scale, out=self.attn, max_kv_len_hint=self.max_len)
+            else:
+                _capi.kv_append(q=q, k=k, v=v, q_out=self.q_out, q_norm_w=lw.q_norm,
+                                k_norm_w=lw.k_norm, eps=lw.qk_eps, cos=cos, sin=sin,
+                                pool=self.pool, slot_rows=rows[l], page_size=P)
+                _capi.paged_decode_attention(self.q_out, self.pool, self.tables[l], lens1,
+                                             num_kv_heads=w.hkv, page_size=P, scale=scale,
+                                             out=self.attn, max_kv_len_hint=self.max_len)
             self._row_proj(self.attn.view(B, w.hq * D), lw.wo, h)
             self._gemv(h, lw.wg, self.act, norm_w=lw.ln2, eps=lw.eps2, w2=lw.wu)
             self._row_proj(self.act, lw.wd, h)
         self._gemv(h, w.lm_head, self.logits, norm_w=w.final_norm, eps=w.final_eps)
-        # greedy pick over the vocab shards: (max value, global index) per rank
+        if self.sampler is not None:
+            nxt = self.sampler(self.logits if self.world == 1 else self.full_logits()).view(-1)
+        else:
+            nxt = self._greedy()
+        self.next = nxt.long().view(B, 1)
+        if self.fp4:   # a sequence that is idle keeps its token
+            self.next = torch.where(self.new_lens.view(B, 1) > 0, self.next, self.ids)
+        self.lens.copy_(lens1)
+        self.ids.copy_(self.next if forced is None else forced)
+
+    def _greedy(self) -> torch.Tensor:
+        """Greedy pick over the vocab shards: (max value, global index) per rank."""
+        B = self.B
         val, idx = self.logits.float().max(dim=-1)
-        local = torch.stack([val, (idx + self.rank * w.lm_head.shape[0]).float()], dim=-1)
+        local = torch.stack([val, (idx + self.rank * self.w.lm_head.shape[0]).float()], dim=-1)
         if self.world > 1:
             dist.all_gather_into_tensor(self.pick.view(-1), local.view(-1).contiguous(),
                                         group=self.group)
             best = self.pick[:, :, 0].argmax(dim=0)          # first rank wins ties
-            nxt = self.pick[best, torch.arange(B, device=self.dev), 1]
-        else:
-            nxt = local[:, 1]
-        self.next = nxt.long().view(B, 1)
-        self.lens.copy_(lens1)
-        self.ids.copy_(self.next if forced is None else forced)
+            return self.pick[best, torch.arange(B, device=self.dev), 1]
+        return local[:, 1]
 
     def capture(self) -> None:
         """Captures step() (argmax feeding the next step) as a CUDA graph."""
@@ -307,7 +402,7 @@ class TPDecodeModel:
         saved = (self.lens.clone(), self.ids.clone())
         with torch.cuda.stream(side), _capi.decode_overlap():
             with torch.cuda.graph(g, stream=side):
-                self.step()
+                self._step()
         torch.cuda.current_stream(self.dev).wait_stream(side)
         torch.cuda.synchronize(self.dev)
         self.lens.copy_(saved[0])
@@ -315,6 +410,8 @@ class TPDecodeModel:
         self.graph = g
 
     def replay(self) -> None:
+        if self.sampler is not None:
+            self.sampler.tick()
         self.graph.replay()
 
     def full_logits(self) -> torch.Tensor:
