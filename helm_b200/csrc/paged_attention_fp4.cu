@@ -65,7 +65,7 @@ struct DecodeFp4Args {
   int num_workers;
   int early;         // decode overlap: the lengths and tables may be read before the wait
   float score_scale; // softmax scale x K cache scale
-  float softcap;
+  float softcap, softcap_inv;
   float v_scale;
   // A state's maximum m is in log2 units in the plain form (no mask, no softcap,
   // scale > 0), in natural units of the score otherwise (a mask of the type's
@@ -97,6 +97,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// tanh without a branch: its odd series to x^11 below 1/4 (next term 2e-10), else
+// 1 - 2 / (e^2x + 1) (3e-7 absolute).
+__device__ __forceinline__ float tanh_fast(float x) {
+  const float z = x * x;
+  float p = fmaf(z, -1382.f / 155925.f, 62.f / 2835.f);
+  p = fmaf(p, z, -17.f / 315.f);
+  p = fmaf(p, z, 2.f / 15.f);
+  p = fmaf(p, z, -1.f / 3.f);
+  const float small = fmaf(p * z, x, x);
+  const float e = exp2_fast(fabsf(x) * (2.f * kLog2e));  // inf: 1
+  const float large = copysignf(1.f - __fdividef(2.f, e + 1.f), x);
+  return z < 0.0625f ? small : (e < INFINITY ? large : copysignf(1.f, x));
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint64_t* bar) {
@@ -488,6 +502,18 @@ struct Fp4Worker {
   template <bool kFull>
   __device__ __forceinline__ void unit(const DecodeFp4Args& a, uint32_t base, int valid, int tok0,
                                        int lane) {
+    // mask values of this lane's tokens (rows A and B of both tiles): asked for
+    // before the products, used after them
+    float mask[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    const bool masked = !kFull && !kPlain && a.mask != nullptr;
+    if (masked) {
+      const int r = lane >> 2, first = 4 * (r >> 1) + (r & 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = (i >> 1) * kFp4TileTokens + first + 2 * (i & 1);
+        mask[i >> 1][i & 1] = t < valid ? fp4_mask(a, cur_b, tok0 + t) : -INFINITY;
+      }
+    }
     float s[2][NT][4];
     scores(base, s[0]);
     scores(base + L::kBytes, s[1]);
@@ -500,7 +526,7 @@ struct Fp4Worker {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = s[ti][nt][e] * cx[nt][e & 1];
-            if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+            if (a.softcap > 0.f) x = a.softcap * tanh_fast(x * a.softcap_inv);
             s[ti][nt][e] = x;
           }
     }
@@ -511,10 +537,8 @@ struct Fp4Worker {
       for (int ti = 0; ti < 2; ++ti) {
         const int v = valid - ti * kFp4TileTokens;
         bool seeA = tA < v, seeB = tB < v;
-        if (!kPlain && a.mask != nullptr) {
-          const int t0 = tok0 + ti * kFp4TileTokens;
-          const float mA = seeA ? fp4_mask(a, cur_b, t0 + tA) : -INFINITY;
-          const float mB = seeB ? fp4_mask(a, cur_b, t0 + tB) : -INFINITY;
+        if (masked) {
+          const float mA = mask[ti][0], mB = mask[ti][1];
           seeA = mA != -INFINITY;
           seeB = mB != -INFINITY;
 #pragma unroll
@@ -1023,6 +1047,7 @@ extern "C" int helm_paged_decode_attention_fp4(
   const bool plain = mask == nullptr && !(softcap > 0.f) && scale > 0.f;
   a.score_scale = scale * k_scale;
   a.softcap = softcap;
+  a.softcap_inv = softcap > 0.f ? 1.f / softcap : 0.f;
   a.v_scale = v_scale;
   a.unit_log2 = plain ? 1.f : kLog2e;
   a.unit_ln = plain ? kLn2 : 1.f;
