@@ -19,11 +19,12 @@
 // With few rows a row is held by one cluster, its logits in the CTAs' shared
 // memory.  With at least as many rows as SMs one CTA does a row, reading it from
 // L2 once per pass: no cluster barriers, and two rows share an SM, one computing
-// while the other waits (256 x 151936: 197 -> @BIG@ us).  A filter needs its last kept candidate.  A histogram of counts
+// while the other waits (256 x 151936 bf16: top-k 144 -> 94 us, no filter 127 ->
+// 93).  A filter needs its last kept candidate.  A histogram of counts
 // over 2048 equal steps of the logit (equal steps spread a bell-shaped row over
 // the bins; digits of its bit pattern would not) says in which bin it falls:
 // exactly for top-k, and for top-p by an estimate from counts times the weight at
-// the bins' centres, good to a few bins (a window of 32 is kept around it).  Then
+// the bins' centres, good to a few bins (a window of 8 bins, or of 64 candidates, is kept around it).  Then
 //   few: when at most 1024 candidates lie in that bin (window) or above, they are
 //        sorted in one CTA, which finishes the row; the others are done;
 //   many: one pass in fp64 sums the weights above the window, per warp, and each
@@ -48,7 +49,8 @@ namespace cg = cooperative_groups;
 constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kSampBins = 2048;
-constexpr int kSampWindow = 32;              // bins around the estimate of top-p's cut
+constexpr int kSampWindow = 8;               // bins around the estimate of top-p's cut
+constexpr int kSampMargin = 64;              // candidates beyond it that few-candidate rows sort too
 constexpr int kSampList = 1024;              // candidates sorted in one CTA
 constexpr int kSampMaxVocab = 1 << 18;       // 2^18 weights of 2^44 stay below 2^63
 constexpr int kSampSliceBytes = 160 * 1024;  // most logits a CTA can hold
@@ -154,7 +156,9 @@ struct __align__(16) SampleShared {
   uint32_t pub_n;
   // results, the same for every CTA of the cluster
   int bin_k, bin_p;               // bins of the filters' last candidates (bin_p: estimate)
-  uint32_t upto_k, in_k, upto_w;  // candidates up to and in bin_k; up to the window's end
+  uint32_t upto_k, in_k;          // candidates up to and in bin_k
+  uint32_t upto_p, upto_w, upto_f;  // up to bin_p, up to the window's end, up to bin_f
+  int bin_f;                      // bin with kSampMargin candidates beyond bin_p
   uint32_t win_lo[kSampWindow], win_hi[kSampWindow];  // weights of the window's bins
   int win_bin;                    // the window's bin that the weights point to
   u64 win_over;                   // weight above it
@@ -177,6 +181,7 @@ struct Sampler {
   int vecs;          // 16-byte groups of its slice (padded with -inf)
   int ranks, rank, lane, warp;
   float top;         // largest logit of the row
+  double top_finite;
   double inv_temp, scale;  // z = (l - l_max) inv_temp, y = (l - l_max) scale
   float bin_scale;
   float least_logit;  // below it weights round to 0
@@ -189,12 +194,21 @@ struct Sampler {
     rank = static_cast<int>(cluster.block_rank());
   }
 
+  // (+inf stands for the largest finite float here: infinities share the weight)
   __device__ __forceinline__ u64 weight(float f) const {
-    const u64 w = weight_fixed((static_cast<double>(f) - static_cast<double>(top)) * scale, s.table);
-    return f == top ? u64(1) << 44 : (f >= least_logit ? w : 0);  // -inf is below it
+    const double d = static_cast<double>(fminf(f, 3.402823466e38f)) - top_finite;
+    const u64 w = weight_fixed(d * scale, s.table);
+    return f >= least_logit ? w : 0;  // -inf is below it
+  }
+  // Place on the bins' scale; bin b holds the places from b to b + 1 (with one bin
+  // for all, the places may be NaN: they count as its own).
+  __device__ __forceinline__ float place(float f) const { return (top - f) * bin_scale; }
+  __device__ __forceinline__ static bool between(float x, int b0, int b1) {  // bins b0 .. b1
+    return !(x < static_cast<float>(b0)) &&
+           (!(x >= static_cast<float>(b1 + 1)) || b1 == kSampBins - 1);
   }
   __device__ __forceinline__ int bin(float f) const {
-    return max(0, min(kSampBins - 1, static_cast<int>((top - f) * bin_scale)));
+    return min(kSampBins - 1, static_cast<int>((top - f) * bin_scale));  // f <= top; NaN: 0
   }
   __device__ __forceinline__ uint4 raw(int vec) const {
     const uint4* p = reinterpret_cast<const uint4*>(slice) + vec;
@@ -441,16 +455,33 @@ struct Sampler {
       }
     }
     __syncthreads();
-    if (use_p) {
-      const int end = window_begin() + kSampWindow - 1;
-      before = ex;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        before += c[i];
-        if (b0 + i == end) s.upto_w = before;
-      }
-      __syncthreads();
+    if (!use_p) return;
+    // Where candidates are few and heavy the estimate may be off by the empty bins
+    // between two of them: the margin for sorting goes by candidates.
+    const int end = window_begin() + kSampWindow - 1, at_p = s.bin_p;
+    if (threadIdx.x == 0) {
+      s.bin_f = kSampBins - 1;
+      s.upto_f = total;
     }
+    before = ex;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      before += c[i];
+      if (b0 + i == end) s.upto_w = before;
+      if (b0 + i == at_p) s.upto_p = before;
+    }
+    __syncthreads();
+    const uint32_t goal = s.upto_p + kSampMargin;
+    before = ex;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (before < goal && before + c[i] >= goal) {
+        s.bin_f = b0 + i;
+        s.upto_f = before + c[i];
+      }
+      before += c[i];
+    }
+    __syncthreads();
   }
   __device__ __forceinline__ int window_begin() const {
     return max(0, min(s.bin_p - kSampWindow / 2, kSampBins - kSampWindow));
@@ -459,17 +490,19 @@ struct Sampler {
   // Weights of the whole row, per lane: its sum (total), what lies above bin lo
   // (above) and of that what min-p keeps (kept); the weights of the bins lo ..
   // lo + kSampWindow - 1 are added up in shared memory.
-  __device__ __forceinline__ void weigh(int lo, double least, u64& total, u64& above, u64& kept) {
+  __device__ __forceinline__ void weigh(int lo, u64 least, u64& total, u64& above, u64& kept) {
     if (threadIdx.x < kSampWindow) s.win_lo[threadIdx.x] = s.win_hi[threadIdx.x] = 0;
     __syncthreads();
     const int s1 = seg_begin(warp + 1);
     each(seg_begin(warp) + lane, s1, 32, [&](float f, int) {
       const u64 w = weight(f);
-      const int at = bin(f) - lo;
+      const float at_f = place(f);
+      const bool over = at_f < static_cast<float>(lo);
       total += w;
-      above += at < 0 ? w : 0;
-      kept += at < 0 && (static_cast<double>(w) >= least || f == top) ? w : 0;
-      if (static_cast<unsigned>(at) < static_cast<unsigned>(kSampWindow) && w != 0) {
+      above += over ? w : 0;
+      kept += over && w >= least ? w : 0;
+      if (between(at_f, lo, lo + kSampWindow - 1) && w != 0) {
+        const int at = bin(f) - lo;
         const uint32_t x = static_cast<uint32_t>(w);
         const uint32_t old = atomicAdd(&s.win_lo[at], x);
         const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + x < old ? 1u : 0u);
@@ -485,7 +518,7 @@ struct Sampler {
     __syncthreads();
     if (warp == 0) {
       u64 m = 0;
-      for (int r = 0; r < ranks; ++r) {
+      for (int r = 0; r < ranks && lane < kSampWindow; ++r) {
         const SampleShared* o = cluster.map_shared_rank(&s, r);
         m += (static_cast<u64>(o->win_hi[lane]) << 32) + o->win_lo[lane];
       }
@@ -501,7 +534,7 @@ struct Sampler {
         s.win_over = ex;
       }
     }
-    static_assert(kSampWindow == 32, "");
+    static_assert(kSampWindow <= 32, "");
     __syncthreads();
     over = s.win_over;
     return s.win_bin;
@@ -529,7 +562,7 @@ struct Sampler {
     block_scan(x, s.warp_a, sum);
     return sum;
   }
-  __device__ void alone(int row, float p, double least, float u, u64 row_total) {
+  __device__ void alone(int row, float p, u64 least, float u, u64 row_total) {
     const T* src = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.row_stride;
     const u64 target = top_p_target(p, row_total);
     u64 lo = 0, hi = ~u64(0);
@@ -539,7 +572,7 @@ struct Sampler {
       (m >= target ? lo : hi) = mid;
     }
     auto keep = [&](float f, int i) {
-      return order_of(f, i) >= lo && (static_cast<double>(weight(f)) >= least || f == top);
+      return order_of(f, i) >= lo && weight(f) >= least;
     };
     const u64 goal = draw_goal(u, row_sum(src, keep));
     int first = -1, end = a.vocab - 1;  // the sum up to `end` exceeds the goal, up to `first` not
@@ -608,13 +641,17 @@ struct Sampler {
       cluster.sync();
       return;
     }
+    top_finite = static_cast<double>(fminf(top, 3.402823466e38f));
     inv_temp = greedy ? 1.0 : 1.0 / static_cast<double>(temp);
     scale = 92.332482616893656877 * inv_temp;  // 64 / ln 2
     // bins span the finite logits, at most 64 T (weights below e^-64 vanish)
     least_logit = fmaxf(top - 31.3f * (greedy ? 1.f : temp), -3.402823466e38f);
     const float span = fminf(top - mn, fmaxf(64.f * temp, 32.f));
     bin_scale = span > 0.f && span < INFINITY ? (kSampBins - 1) / span : 0.f;
-    const double least = static_cast<double>(mp) * 17592186044416.0;  // min_p in units of 2^-44
+    // min_p in units of 2^-44; the largest candidates (weight 2^44) always stay
+    const u64 least =
+        mp > 0.f ? min(u64(1) << 44, static_cast<u64>(ceil(static_cast<double>(mp) * 17592186044416.0)))
+                 : 0;
 
     // ---- where the filters cut -------------------------------------------------
     const int s0 = seg_begin(warp), s1 = seg_begin(warp + 1);
@@ -624,14 +661,17 @@ struct Sampler {
     // they fit its list; sums the row where rank 0 needs that: for top-p without
     // top-k and for log probabilities.
     auto try_few = [&](int upto) {
+      // every logit of those bins (and, by rounding, perhaps a few more)
+      const float low = bin_scale > 0.f ? top - (upto + 1) / bin_scale * 1.00001f : -INFINITY;
+      const float from = upto < kSampBins - 1 && low > -3.402823466e38f ? low : -3.402823466e38f;
       if (a.logprobs != nullptr || !use_k) {
         each(s0 + lane, s1, 32, [&](float f, int i) {
           row_total += weight(f);
-          if (f > -INFINITY && bin(f) <= upto) push(home, f, i);
+          if (f >= from) push(home, f, i);
         });
       } else {
         each(s0 + lane, s1, 32, [&](float f, int i) {
-          if (f > -INFINITY && bin(f) <= upto) push(home, f, i);
+          if (f >= from) push(home, f, i);
         });
       }
       cluster_sum(row_total, above);
@@ -652,8 +692,9 @@ struct Sampler {
     }
     if (use_k || use_p) {
       histogram(k, use_k, p, use_p);
-      if ((use_k ? s.upto_k : s.upto_w) <= kSampList &&
-          try_few(use_k ? s.bin_k : window_begin() + kSampWindow - 1))
+      // (top-p alone: the window and the margin, whichever reaches further)
+      if ((use_k ? s.upto_k : max(s.upto_w, s.upto_f)) <= kSampList &&
+          try_few(use_k ? s.bin_k : max(s.bin_f, window_begin() + kSampWindow - 1)))
         return;
     }
 
@@ -671,7 +712,7 @@ struct Sampler {
       each(s0 + lane, s1, 32, [&](float f, int) {
         const u64 w = weight(f);
         row_total += w;
-        warp_kept += static_cast<double>(w) >= least || f == top ? w : 0;
+        warp_kept += w >= least ? w : 0;
       });
       warp_kept = warp_reduce(warp_kept, AddOp());
       cluster_sum(row_total, above);
@@ -731,10 +772,9 @@ struct Sampler {
         // what is kept of the bins lo .. cut joins the sums
         u64 more = 0;
         each(s0 + lane, s1, 32, [&](float f, int i) {
-          const int b = bin(f);
-          if (b >= lo && b <= cut && f > -INFINITY && order_of(f, base + i) >= last) {
+          if (between(place(f), lo, cut) && f > -INFINITY && order_of(f, base + i) >= last) {
             const u64 w = weight(f);
-            more += static_cast<double>(w) >= least || f == top ? w : 0;
+            more += w >= least ? w : 0;
           }
         });
         warp_kept += warp_reduce(more, AddOp());
@@ -748,7 +788,7 @@ struct Sampler {
       if (greedy) return f == top ? 1 : 0;
       if (last != 0 && order_of(f, base + i) < last) return 0;
       const u64 w = weight(f);
-      return static_cast<double>(w) >= least || f == top ? w : 0;
+      return w >= least ? w : 0;
     };
     if (!known) {
       u64 x = 0;
@@ -804,7 +844,7 @@ struct Sampler {
   }
 
   // Rank 0, its list holding every candidate that may be kept: the row's token.
-  __device__ void finish_few(int row, int k, bool use_k, float p, bool use_p, double least, float u,
+  __device__ void finish_few(int row, int k, bool use_k, float p, bool use_p, u64 least, float u,
                              u64 row_total) {
     const int count = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kSampList)));
     u64 w[2], ex[2], sum;
@@ -832,7 +872,7 @@ struct Sampler {
     for (int i = 0; i < 2; ++i) {
       const int at = 2 * threadIdx.x + i;
       const bool keep = at < count && (!use_k || at < k) && ex[i] < target &&
-                        (static_cast<double>(w[i]) >= least || w[i] == u64(1) << 44);
+                        w[i] >= least;
       const u64 entry = at < count ? s.list[at] : 0;
       value[i] = key_value(static_cast<uint32_t>(entry >> 32));
       if (keep) key[i] = (entry << 32) | static_cast<u64>(at) | 0x80000000ull;
@@ -879,7 +919,7 @@ struct Sampler {
     cluster.sync();
     SampleShared* home = cluster.map_shared_rank(&s, 0);
     each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
-      if (f > -INFINITY && bin(f) == which) push(home, f, i);
+      if (between(place(f), which, which) && f > -INFINITY) push(home, f, i);
     });
     cluster.sync();
     if (rank == 0) {
