@@ -20,11 +20,14 @@
 // memory.  With at least as many rows as SMs one CTA does a row, reading it from
 // L2 once per pass: no cluster barriers, and two rows share an SM, one computing
 // while the other waits (256 x 151936 bf16: top-k 144 -> 94 us, no filter 127 ->
-// 93).  A filter needs its last kept candidate.  A histogram of counts
-// over 2048 equal steps of the logit (equal steps spread a bell-shaped row over
-// the bins; digits of its bit pattern would not) says in which bin it falls:
-// exactly for top-k, and for top-p by an estimate from counts times the weight at
-// the bins' centres, good to a few bins (a window of 8 bins, or of 64 candidates, is kept around it).  Then
+// 93).  Bound by instructions: some 30 per logit for its weight, 10 for a bin.
+//
+// A filter needs its last kept candidate.  A histogram of counts over 2048 equal
+// steps of the logit (equal steps spread a bell-shaped row over the bins; digits
+// of its bit pattern would not) says in which bin it falls: exactly for top-k, and
+// for top-p by an estimate from counts times the weight at the bins' centres, good
+// to a bin or two among many candidates (a window of 8 bins is kept around it, a
+// margin of 64 candidates where they are few).  Then
 //   few: when at most 1024 candidates lie in that bin (window) or above, they are
 //        sorted in one CTA, which finishes the row; the others are done;
 //   many: one pass in fp64 sums the weights above the window, per warp, and each
@@ -489,20 +492,23 @@ struct Sampler {
 
   // Weights of the whole row, per lane: its sum (total), what lies above bin lo
   // (above) and of that what min-p keeps (kept); the weights of the bins lo ..
-  // lo + kSampWindow - 1 are added up in shared memory.
-  __device__ __forceinline__ void weigh(int lo, u64 least, u64& total, u64& above, u64& kept) {
+  // lo + kSampWindow - 1 are added up in shared memory, the candidates of bin
+  // `which` sent to rank 0's (empty) list.
+  __device__ __forceinline__ void weigh(int lo, int which, u64 least, u64& total, u64& above, u64& kept) {
     if (threadIdx.x < kSampWindow) s.win_lo[threadIdx.x] = s.win_hi[threadIdx.x] = 0;
     __syncthreads();
     const int s1 = seg_begin(warp + 1);
-    each(seg_begin(warp) + lane, s1, 32, [&](float f, int) {
+    SampleShared* home = cluster.map_shared_rank(&s, 0);
+    each(seg_begin(warp) + lane, s1, 32, [&](float f, int i) {
       const u64 w = weight(f);
       const float at_f = place(f);
       const bool over = at_f < static_cast<float>(lo);
       total += w;
       above += over ? w : 0;
       kept += over && w >= least ? w : 0;
-      if (between(at_f, lo, lo + kSampWindow - 1) && w != 0) {
+      if (between(at_f, lo, lo + kSampWindow - 1) && f > -INFINITY) {
         const int at = bin(f) - lo;
+        if (at + lo == which) push(home, f, i);
         const uint32_t x = static_cast<uint32_t>(w);
         const uint32_t old = atomicAdd(&s.win_lo[at], x);
         const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + x < old ? 1u : 0u);
@@ -675,8 +681,11 @@ struct Sampler {
         });
       }
       cluster_sum(row_total, above);
-      if (home->list_n > kSampList) {
+      if (home->list_n > kSampList) {  // (seen by all alike)
         row_total = above = 0;
+        cluster.sync();
+        if (threadIdx.x == 0) s.list_n = 0;
+        cluster.sync();
         return false;
       }
       cluster.sync();  // all have seen the count: rank 0 may use its list, the others leave
@@ -685,10 +694,9 @@ struct Sampler {
     };
     if (use_k && k <= ranks * (kSampThreads / 4)) {
       if (try_few(bound_k(own_max, k))) return;
-      cluster.sync();  // more than the list holds: start over with all logits
+      // more than the list holds: start over with all logits
       for (int i = threadIdx.x; i < kSampBins; i += kSampThreads) s.hist[i] = 0;
-      if (threadIdx.x == 0) s.list_n = 0;
-      cluster.sync();
+      __syncthreads();
     }
     if (use_k || use_p) {
       histogram(k, use_k, p, use_p);
@@ -720,7 +728,7 @@ struct Sampler {
       // Many candidates.  top-k first: its bin is exact.
       u64 mass = 0;
       int lo = use_k ? min(s.bin_k, kSampBins - kSampWindow) : window_begin();
-      weigh(lo, least, row_total, above, warp_kept);
+      weigh(lo, use_k ? s.bin_k : s.bin_p, least, row_total, above, warp_kept);
       warp_kept = warp_reduce(warp_kept, AddOp());
       cluster_sum(row_total, above);
       mass = row_total;
@@ -733,7 +741,7 @@ struct Sampler {
               const SampleShared* o = cluster.map_shared_rank(&s, r);
               over += (static_cast<u64>(o->win_hi[b - lo]) << 32) + o->win_lo[b - lo];
             }
-          last = bin_last(s.bin_k, false, static_cast<u64>(k) - (s.upto_k - s.in_k), over, mass);
+          last = bin_last(s.bin_k, true, false, static_cast<u64>(k) - (s.upto_k - s.in_k), over, mass);
           cut = s.bin_k;
         } else {
           last = bisect(false, static_cast<u64>(k), mass);
@@ -742,11 +750,12 @@ struct Sampler {
       }
       if (use_p) {
         if (use_k) {  // the sums were taken at top-k's bin: again at top-p's
+          if (threadIdx.x == 0) s.list_n = 0;
           cluster.sync();
           lo = window_begin();
           u64 again = 0;
           above = warp_kept = 0;
-          weigh(lo, least, again, above, warp_kept);
+          weigh(lo, s.bin_p, least, again, above, warp_kept);
           warp_kept = warp_reduce(warp_kept, AddOp());
           cluster_sum(again, above);
           known = true;
@@ -758,7 +767,7 @@ struct Sampler {
         if (found >= 0)
           for (int r = 0; r < ranks; ++r) in_bin += cluster.map_shared_rank(&s, r)->hist[found];
         if (found >= 0 && in_bin <= kSampList) {
-          by_p = bin_last(found, true, target - over, over, m);
+          by_p = bin_last(found, found == s.bin_p, true, target - over, over, m);
           cut = found;
         }
         if (by_p == 0) {
@@ -914,14 +923,18 @@ struct Sampler {
   // The order of the last kept candidate within a bin of at most kSampList
   // candidates, where `need` more (counted or weighed) are to be kept; mass =
   // above + the bin's weight up to it.  0 when the bin does not hold enough.
-  __device__ u64 bin_last(int which, bool by_mass, u64 need, u64 above, u64& mass) {
-    if (rank == 0 && threadIdx.x == 0) s.list_n = 0;
-    cluster.sync();
-    SampleShared* home = cluster.map_shared_rank(&s, 0);
-    each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
-      if (between(place(f), which, which) && f > -INFINITY) push(home, f, i);
-    });
-    cluster.sync();
+  // listed: rank 0's list holds the bin's candidates already.
+  __device__ u64 bin_last(int which, bool listed, bool by_mass, u64 need, u64 above, u64& mass) {
+    if (!listed) {
+      cluster.sync();
+      if (threadIdx.x == 0) s.list_n = 0;
+      cluster.sync();
+      SampleShared* home = cluster.map_shared_rank(&s, 0);
+      each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
+        if (between(place(f), which, which) && f > -INFINITY) push(home, f, i);
+      });
+      cluster.sync();
+    }
     if (rank == 0) {
       const int count = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kSampList)));
       u64 w[2], ex[2], sum;

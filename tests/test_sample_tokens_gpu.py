@@ -176,6 +176,32 @@ def test_captured_and_replayed(dev):
                                                  top_p=float(np.float32(0.8)))[0]
 
 
+def test_border_of_the_sorted_list(dev):
+    """Exactly as many candidates up to the k-th one's bin as are sorted in one go, and more of
+    them within rounding of that bin's edge: they do not fit, and the row takes the long way."""
+    v = 3000
+    x = torch.full((2, v), -60.0)
+    x[:, 0] = 10.0
+    x[:, 1:1024] = 10.0 - 0.6
+    edge = 20 / (2047 / 64)   # the bins are 64 / 2047 wide; 0.6 lies in the 20th
+    x[:, 1024:1080] = float(np.float32(10.0 - edge * (1 + 5e-6)))
+    u = [0.3, 0.9]
+    _check(dev, x.to(dev), u, top_k=[1024, 1024])
+    _check(dev, x.to(dev), u, top_k=[1024, 1050], top_p=[0.9, 0.99])
+
+
+def test_few_heavy_candidates_with_gaps(dev):
+    """Top-p's share ends next to a gap of many empty bins: the estimate may fall on either side."""
+    x = torch.full((40, 5000), -20.0)
+    x[:, ::50] = 6.0 - 0.21 * torch.arange(100)
+    l = x.double().numpy()
+    w = np.sort(np.exp(l[0] - l[0].max()))[::-1].cumsum() / np.exp(l[0] - l[0].max()).sum()
+    # shares just below and above the running sums of the first candidates
+    p = [float(np.float32(w[i // 2] * (1 + (1e-3 if i % 2 else -1e-3)))) for i in range(40)]
+    g = torch.Generator().manual_seed(3)
+    _check(dev, x.to(dev), torch.rand(40, generator=g).tolist(), top_p=[min(q, 0.9999) for q in p])
+
+
 def test_wrapper_refusals(dev):
     x, u = torch.zeros(2, 8, device=dev), torch.zeros(2, device=dev)
     for bad in (lambda: _capi.sample_tokens(x.t(), u), lambda: _capi.sample_tokens(x, u[:1]),
