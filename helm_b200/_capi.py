@@ -97,7 +97,7 @@ _SIGNATURES = {
         _P, _I64, _I64,            # q, strides
         _P, _I64,                  # pool, pool_pages
         _P, _I64, _I, _P,          # page_table, pt_stride_b, max_pages, kv_lens
-        _P, _I, _I64,              # mask, mask_dtype, mask_stride_b
+        _P, _I, _I64, _I64,        # mask, mask_dtype, mask_stride_b, mask_len
         _P, _I64, _I64, _P,        # out, strides, lse
         _P, _I64,                  # workspace, bytes
         _I, _I, _I, _I, _I, _I,    # batch, hq, hkv, head_dim, page_size, dtype
@@ -754,6 +754,8 @@ def kv_append_fp4(*, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor,
     for w in (q_norm_w, k_norm_w):
         if w is not None and (w.shape != (D,) or w.dtype is not dt or not w.is_contiguous()):
             _refuse(what, "norm weights must be contiguous [D] of k's dtype")
+    if N == 0:  # (empty tensors have no address)
+        return
     rc = _call(idx, (_lib or lib()).helm_kv_append_fp4, qp, qst, qsh, k.data_ptr(), ks[0], ks[1],
                v.data_ptr(), vs[0], vs[1], _ptr(q_norm_w), _ptr(k_norm_w), eps, _ptr(cos),
                _ptr(sin), rs, qop, qot, qoh, pool.data_ptr(), pool.shape[0], slot_rows.data_ptr(),
@@ -791,6 +793,8 @@ def gather_kv_rows_fp4(pool: torch.Tensor, slot_rows: torch.Tensor, *, page_size
     if (k_out.shape != shape or v_out.shape != shape or k_out.dtype is not dtype
             or v_out.dtype is not dtype or ks[2] != 1 or vs[2] != 1):
         _refuse(what, "outputs must be [N, Hkv, D] in dtype with a unit dim stride")
+    if N == 0:
+        return k_out, v_out
     rc = _call(idx, (_lib or lib()).helm_gather_kv_rows_fp4, pool.data_ptr(), pages,
                slot_rows.data_ptr(), k_out.data_ptr(), ks[0], ks[1], v_out.data_ptr(), vs[0],
                vs[1], N, Hkv, D, page_size, helm_dtype(dtype), k_scale, v_scale,
@@ -813,7 +817,8 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
     """Decode attention over a pool of 4-bit pages (fp4_pool).
 
     q [B, Hq, D] (dim stride 1); page_table int32 [B, max_pages]; kv_lens int32
-    [B]; mask additive [B or 1, T] with T >= max(kv_lens), -inf excludes a key.
+    [B]; mask additive [B or 1, T], -inf excludes a key.  A length beyond T or
+    the table's row is cut and HELM_DEV_BAD_PAGE recorded (device_status).
     Returns (out [B, Hq, D] in q.dtype, lse fp32 [B, Hq] or None).
     """
     what = "paged_decode_attention_fp4"
@@ -844,12 +849,14 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
         if lse.dtype is not torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous():
             _refuse(what, "lse must be contiguous fp32 [B, Hq]")
         lse_ptr = lse.data_ptr()
-    mask_ptr, mask_dt, mask_sb = None, 0, 0
+    mask_ptr, mask_dt, mask_sb, mask_len = None, 0, 0, 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] not in (1, B):
-            _refuse(what, "mask must be [B or 1, T]")
+        if mask.dim() != 2 or mask.shape[0] not in (1, B) or mask.shape[1] < 1:
+            _refuse(what, "mask must be [B or 1, T], T >= 1")
         if mask.stride(1) != 1:
-            mask = mask.contiguous()
+            with torch.cuda.stream(stream):  # (None: the current one)
+                mask = mask.contiguous()
+        mask_len = mask.shape[1]
         mask_ptr, mask_dt = mask.data_ptr(), helm_dtype(mask.dtype)
         mask_sb = mask.stride(0) if mask.shape[0] > 1 else 0
     L = _lib or lib()
@@ -864,8 +871,8 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
         ws.record_stream(stream)
     rc = _call(idx, L.helm_paged_decode_attention_fp4, q.data_ptr(), qs[0], qs[1], pool.data_ptr(),
                pool.shape[0], page_table.data_ptr(), ts[0], tshape[1], kv_lens.data_ptr(),
-               mask_ptr, mask_dt, mask_sb, out.data_ptr(), os_[0], os_[1], lse_ptr, ws.data_ptr(),
-               nbytes, B, Hq, num_kv_heads, D, page_size, helm_dtype(dt), scale, softcap or 0.0,
+               mask_ptr, mask_dt, mask_sb, mask_len, out.data_ptr(), os_[0], os_[1], lse_ptr,
+               ws.data_ptr(), nbytes, B, Hq, num_kv_heads, D, page_size, helm_dtype(dt), scale, softcap or 0.0,
                k_scale, v_scale, max_kv_len_hint, _stream_of(idx, stream))
     if rc:
         _check(rc, "helm_paged_decode_attention_fp4")

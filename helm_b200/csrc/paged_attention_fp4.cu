@@ -48,7 +48,7 @@ struct DecodeFp4Args {
   int64_t pool_pages;
   const int32_t* page_table;
   int64_t pt_sb;
-  int max_pages;
+  int most;  // tokens that a row of the table, and of the mask, can describe
   const int32_t* kv_lens;
   const void* mask;
   int mask_dtype;
@@ -156,13 +156,13 @@ __device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Tokens of sequence b (a length beyond its row of the table is cut and reported).
+// Tokens of sequence b (a length beyond its row of the table, or of the mask, is
+// cut and reported).
 __device__ __forceinline__ int fp4_len(const DecodeFp4Args& a, int b) {
   const int len = a.kv_lens[b];
-  const int64_t most = static_cast<int64_t>(a.max_pages) * a.page_size;
-  if (len > most) {
+  if (len > a.most) {
     report_status(HELM_DEV_BAD_PAGE);
-    return static_cast<int>(most);
+    return a.most;
   }
   return max(len, 0);
 }
@@ -978,8 +978,8 @@ extern "C" int64_t helm_paged_decode_fp4_workspace_bytes(int batch, int num_q_he
 extern "C" int helm_paged_decode_attention_fp4(
     const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* kv_pool, int64_t pool_pages,
     const int32_t* page_table, int64_t pt_stride_b, int max_pages, const int32_t* kv_lens,
-    const void* mask, int mask_dtype, int64_t mask_stride_b, void* out, int64_t out_stride_b,
-    int64_t out_stride_h, float* lse, void* workspace, int64_t workspace_bytes, int batch,
+    const void* mask, int mask_dtype, int64_t mask_stride_b, int64_t mask_len, void* out,
+    int64_t out_stride_b, int64_t out_stride_h, float* lse, void* workspace, int64_t workspace_bytes, int batch,
     int num_q_heads, int num_kv_heads, int head_dim, int page_size, int dtype, float scale,
     float softcap, float k_scale, float v_scale, int max_kv_len_hint, void* stream) {
   using namespace helm;
@@ -990,6 +990,7 @@ extern "C" int helm_paged_decode_attention_fp4(
       pool_pages <= 0 || num_q_heads % num_kv_heads != 0)
     return HELM_ERR_INVALID_ARGUMENT;
   if (!fp4_scale_ok(k_scale) || !fp4_scale_ok(v_scale)) return HELM_ERR_INVALID_ARGUMENT;
+  if (mask != nullptr && mask_len < 0) return HELM_ERR_INVALID_ARGUMENT;
   if (mask != nullptr && mask_dtype != HELM_DTYPE_FP32 && mask_dtype != HELM_DTYPE_BF16 &&
       mask_dtype != HELM_DTYPE_FP16)
     return HELM_ERR_INVALID_ARGUMENT;
@@ -1020,7 +1021,9 @@ extern "C" int helm_paged_decode_attention_fp4(
   a.pool_pages = pool_pages;
   a.page_table = page_table;
   a.pt_sb = pt_stride_b;
-  a.max_pages = max_pages;
+  int64_t tokens = static_cast<int64_t>(max_pages) * page_size;
+  if (mask != nullptr) tokens = std::min(tokens, mask_len);
+  a.most = static_cast<int>(tokens);
   a.kv_lens = kv_lens;
   a.mask = mask;
   a.mask_dtype = mask_dtype;
@@ -1052,7 +1055,6 @@ extern "C" int helm_paged_decode_attention_fp4(
   a.unit_log2 = plain ? 1.f : kLog2e;
   a.unit_ln = plain ? kLn2 : 1.f;
   // bound on the units of the call: it sizes the grid
-  int64_t tokens = static_cast<int64_t>(max_pages) * page_size;
   if (max_kv_len_hint > 0) tokens = std::min<int64_t>(tokens, max_kv_len_hint);
   const int64_t units = (tokens + kUnitTokens - 1) / kUnitTokens * batch * num_kv_heads;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -49,6 +49,12 @@ struct StepArgs {
 
 constexpr uint8_t kStepLeaves = 1, kStepTooLong = 2;
 
+// Sum of two token counts, saturating: the running sums stay in order whatever
+// the lengths are.  (Page counts are bounded by batch * max_pages.)
+__device__ __forceinline__ int token_sum(int a, int b) {
+  return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), 0x7fffffffu));
+}
+
 // Largest b in [0, n) with prefix[b] <= x, for a nondecreasing prefix with
 // prefix[0] = 0 (of equal entries the last: requests that own nothing are skipped).
 __device__ __forceinline__ int owner_of(const int* prefix, int n, int x) {
@@ -98,10 +104,10 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepArg
       flag = kStepLeaves;
       sum[2] += min(held, static_cast<unsigned>(a.max_pages));
     } else if (all <= static_cast<unsigned>(a.max_pages)) {
-      sum[0] += n;
+      sum[0] = token_sum(sum[0], n);
       sum[1] += all - held;
     } else {
-      sum[0] += n;
+      sum[0] = token_sum(sum[0], n);
       flag = kStepTooLong;
     }
     s_past[b] = static_cast<int>(past);
@@ -115,10 +121,11 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepArg
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v += x;
+      if (lane >= off) v = i == 0 ? token_sum(v, x) : v + x;
     }
     if (lane == 31) s_warp[i][warp] = v;
-    before[i] = v - sum[i];
+    v = __shfl_up_sync(0xffffffffu, v, 1);
+    before[i] = lane ? v : 0;
   }
   __syncthreads();
   const int warps = (blockDim.x + 31) / 32;
@@ -129,13 +136,14 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepArg
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v += x;
+      if (lane >= off) v = i == 0 ? token_sum(v, x) : v + x;
     }
     total[i] = __shfl_sync(0xffffffffu, v, 31);
-    before[i] += __shfl_sync(0xffffffffu, v - w, warp);
+    const int warps_before = __shfl_sync(0xffffffffu, v, max(warp - 1, 0));
+    if (warp > 0) before[i] = i == 0 ? token_sum(before[i], warps_before) : before[i] + warps_before;
   }
   for (int b = b0; b < b1; ++b) {
-    s_cu[b] += before[0];
+    s_cu[b] = token_sum(s_cu[b], before[0]);
     s_want[b] += before[1];
     s_give[b] += before[2];
   }
@@ -315,7 +323,8 @@ extern "C" int helm_build_step_tables(const int32_t* past_lens, const int32_t* n
                                       int page_size, int num_rows, void* stream) {
   using namespace helm;
   if (past_lens == nullptr || new_lens == nullptr || page_table == nullptr ||
-      free_pages == nullptr || free_count == nullptr || free_count_out == nullptr ||
+      (free_pages == nullptr && free_capacity > 0) || free_count == nullptr ||
+      free_count_out == nullptr ||
       kv_lens == nullptr || cu_tokens == nullptr || (slot_rows == nullptr && num_rows > 0))
     return HELM_ERR_INVALID_ARGUMENT;
   if (batch <= 0 || page_size <= 0 || max_pages <= 0 || free_capacity < 0 || num_rows < 0 ||

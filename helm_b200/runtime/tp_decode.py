@@ -262,12 +262,17 @@ class TPDecodeModel:
             self.pool.normal_(generator=g)
             self.lens.fill_(length)
             return
-        rows = _capi.build_step_tables(
-            self.lens, (length - self.lens).int(), self.table, self.free_pages, self.free_count,
-            page_size=self.P, num_rows=self.B * length, kv_lens=self.lens)[4]
+
+        def step(new_lens, num_rows):
+            return _capi.build_step_tables(
+                self.lens, new_lens, self.table, self.free_pages, self.free_count,
+                page_size=self.P, num_rows=num_rows, kv_lens=self.lens)[4]
+
+        step(torch.full_like(self.lens, -1), 0)  # what they held goes back
+        rows = step(torch.full_like(self.lens, length), self.B * length)
         if _capi.device_status(self.dev) & _capi.DEV_NO_PAGES:
             raise ValueError("context does not fit the pages")
-        shape = (min(16384, rows.numel()), self.w.hkv, self.D)
+        shape = (max(1, min(16384, rows.numel())), self.w.hkv, self.D)
         for pool in self.pools:
             k, v = (torch.randn(shape, generator=g, device=self.dev).to(self.dtype) for _ in range(2))
             for at in range(0, rows.numel(), shape[0]):

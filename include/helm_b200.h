@@ -117,9 +117,9 @@ int helm_paged_decode_attention(const void* q, int64_t q_stride_b, int64_t q_str
 
 /*
  * Decode overlap, a setting of the calling host thread (default off; returns
- * the previous setting).  When on, helm_paged_decode_attention and
- * helm_paged_decode_attention_noalloc launch the decode kernel as a
- * programmatic dependent of the kernel before it on the stream (PDL): the
+ * the previous setting).  When on, helm_paged_decode_attention,
+ * helm_paged_decode_attention_noalloc and helm_paged_decode_attention_fp4 launch
+ * the decode kernel as a programmatic dependent of the kernel before it on the stream (PDL): the
  * kernel is placed while that one still runs, reads kv_lens, num_pages and
  * page_table and starts loading K/V tiles outside each sequence's last page
  * early, but waits for it to finish before it reads q, the mask or a last
@@ -423,7 +423,9 @@ int helm_gather_kv_rows_fp4(const void* kv_pool, int64_t pool_pages, const int64
  * overlap setting, without ragged page lists (page i of sequence b holds
  * tokens i*page_size ..), O in the query dtype.  A key whose mask value is -inf
  * contributes nothing, whatever its page holds, NaN included; a row that sees
- * no key gets O = 0, LSE = -inf.  q: 4-byte aligned, even strides.
+ * no key gets O = 0, LSE = -inf.  q: 4-byte aligned, even strides.  mask_len:
+ * values in a row of the mask; a length beyond it, or beyond the page table's
+ * row, is cut and HELM_DEV_BAD_PAGE recorded.
  *  workspace  >= helm_paged_decode_fp4_workspace_bytes(...) bytes, 256-byte
  *             aligned, any contents; calls that overlap on the GPU need one each
  */
@@ -433,9 +435,9 @@ int helm_paged_decode_attention_fp4(const void* q, int64_t q_stride_b, int64_t q
                                     const void* kv_pool, int64_t pool_pages,
                                     const int32_t* page_table, int64_t pt_stride_b, int max_pages,
                                     const int32_t* kv_lens, const void* mask, int mask_dtype,
-                                    int64_t mask_stride_b, void* out, int64_t out_stride_b,
-                                    int64_t out_stride_h, float* lse, void* workspace,
-                                    int64_t workspace_bytes, int batch, int num_q_heads,
+                                    int64_t mask_stride_b, int64_t mask_len, void* out,
+                                    int64_t out_stride_b, int64_t out_stride_h, float* lse,
+                                    void* workspace, int64_t workspace_bytes, int batch, int num_q_heads,
                                     int num_kv_heads, int head_dim, int page_size, int dtype,
                                     float scale, float softcap, float k_scale, float v_scale,
                                     int max_kv_len_hint, void* stream);
@@ -463,7 +465,8 @@ int helm_paged_decode_attention_fp4(const void* q, int64_t q_stride_b, int64_t q
  * included) exceed the free ones: its length and pages stay, its tokens' rows
  * are -1, and HELM_DEV_NO_PAGES is recorded.  free_count_out apart, a repeated
  * call with the same inputs gives the same outputs.  B <= 8192;
- * B * max_pages, max_pages * page_size and the sum of new_lens below 2^31.
+ * B * max_pages, max_pages * page_size and the sum of new_lens below 2^31 (a
+ * larger sum saturates).
  *
  * Replaces the host bookkeeping of KVAllocator.allocate / free
  * (helm/runtime/kv_allocator.py:36-93) where a step runs without the host.

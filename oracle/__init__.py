@@ -9,10 +9,13 @@ bench.py.  Nothing in helm_b200/ imports this package.
                       (kv_allocator.py:6-163, kv_cache.py:88-265), metadata only
   norm_rope.py        Qwen3 QK-RMSNorm + rotate_half RoPE with eager bf16 rounding
   merge.py            (O, LSE) merge over disjoint key ranges
+  fp4.py              4-bit K/V format, page layout and attention in float64 (no reference
+                      counterpart: checked against its own definition)
+  serving.py          step tables and sampling, one request and one row at a time (likewise)
 
 Pinning: tests/golden/ holds fixtures produced by running the reference itself
-(tests/golden/make_golden.py); tests/test_oracle.py checks every restatement
-here against them.
+(tests/golden/make_golden.py); tests/test_oracle.py checks the restatements of
+reference code against them.
 """
 from __future__ import annotations
 

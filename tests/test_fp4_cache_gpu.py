@@ -304,6 +304,32 @@ def test_nan_pages_under_an_inf_mask(dev):
     _check_attention(q, kv, out, lse, 0.1, 0.0, _np(mask))
 
 
+def test_a_mask_shorter_than_the_keys_cuts_them(dev):
+    lens, hq, hkv, d, page = [90, 20], 8, 2, 128, 16
+    q, pool, table, kl, kv = _problem(dev, lens, hq, hkv, d, page, BF16, 19)
+    mask = torch.randn(2, 50, generator=torch.Generator().manual_seed(4))
+    lse = torch.empty(2, hq, device=dev)
+    # (the mask lies across its memory, so that the call has to lay it out anew)
+    across = mask.t().contiguous().to(dev).t()
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    out, _ = _capi.paged_decode_attention_fp4(q, pool, table, kl, num_kv_heads=hkv, page_size=page,
+                                              scale=0.1, mask=across, lse=lse, stream=side)
+    side.synchronize()
+    assert _capi.device_status(dev) == _capi.DEV_BAD_PAGE
+    kv[0] = tuple(x[:50] for x in kv[0])
+    _check_attention(q, kv, out, lse, 0.1, 0.0, _np(mask))
+
+
+def test_no_tokens(dev):
+    pool = _capi.fp4_pool(2, 2, 16, 64, dev)
+    none = torch.empty(0, 2, 64, dtype=BF16, device=dev)
+    rows = torch.empty(0, dtype=torch.long, device=dev)
+    _capi.kv_append_fp4(k=none, v=none, q=none, q_out=none, pool=pool, slot_rows=rows, page_size=16)
+    k, v = _capi.gather_kv_rows_fp4(pool, rows, page_size=16, dtype=FP16)
+    assert k.shape == v.shape == (0, 2, 64) and not pool.any()
+
+
 def test_large_and_tiny_queries(dev):
     """bf16 queries outside fp16's range, and scores whose maximum climbs along the sequence."""
     lens, hq, hkv, d, page = [400], 4, 2, 128, 16

@@ -141,12 +141,12 @@ def test_gather_refusals():
 
 def _decode(**kw):
     a = dict(q=P16, q_sb=4096, q_sh=128, pool=P16, pages=64, pt=P16, pt_sb=19, maxp=19, lens=P16,
-             mask=None, mask_dtype=0, out=P16, ws=P256, ws_bytes=1 << 30, batch=2, hq=32, hkv=8,
-             d=128, page=16, dtype=BF16, ks=1.0, vs=1.0)
+             mask=None, mask_dtype=0, mask_len=304, out=P16, ws=P256, ws_bytes=1 << 30, batch=2,
+             hq=32, hkv=8, d=128, page=16, dtype=BF16, ks=1.0, vs=1.0)
     a.update(kw)
     return _capi.lib().helm_paged_decode_attention_fp4(
         a["q"], a["q_sb"], a["q_sh"], a["pool"], a["pages"], a["pt"], a["pt_sb"], a["maxp"],
-        a["lens"], a["mask"], a["mask_dtype"], 0, a["out"], 4096, 128, None, a["ws"],
+        a["lens"], a["mask"], a["mask_dtype"], 0, a["mask_len"], a["out"], 4096, 128, None, a["ws"],
         a["ws_bytes"], a["batch"], a["hq"], a["hkv"], a["d"], a["page"], a["dtype"], 0.088, 0.0,
         a["ks"], a["vs"], 0, None)
 
@@ -158,6 +158,7 @@ def test_decode_refusals():
     assert _decode(hq=30) == INVALID
     assert _decode(ks=1.5) == INVALID
     assert _decode(mask=P16, mask_dtype=7) == INVALID
+    assert _decode(mask=P16, mask_dtype=BF16, mask_len=-1) == INVALID
     assert _decode(hq=136) == UNSUPPORTED       # GQA group of 17
     assert _decode(batch=2049) == UNSUPPORTED
     assert _decode(d=96) == UNSUPPORTED

@@ -168,6 +168,20 @@ def test_requests_come_and_go_over_shared_pages(dev):
     alone.close()
 
 
+def test_fill_kv_starts_over(dev):
+    w = synthetic_shard(ARCH, 0, 1, torch.bfloat16, dev, seed=2)
+    tp = TPDecodeModel(w, batch=2, max_len=64, page_size=16, kv_format="fp4")
+    for length in (40, 17, 0, 63):
+        tp.fill_kv(length)
+        held = 2 * -(-length // 16)
+        assert tp.lens.tolist() == [length] * 2 and tp.free_count.item() == 8 - held
+        pages = tp.table[:, :held // 2].flatten().tolist() + tp.free_pages[:8 - held].tolist()
+        assert sorted(pages) == list(range(8))
+    tp.step()
+    assert tp.lens.tolist() == [64, 64] and _capi.device_status(dev) == 0
+    tp.close()
+
+
 def test_running_out_of_pages_is_reported(dev):
     w = synthetic_shard(ARCH, 0, 1, torch.bfloat16, dev, seed=2)
     tp = TPDecodeModel(w, batch=2, max_len=64, page_size=16, kv_format="fp4", num_pages=3)

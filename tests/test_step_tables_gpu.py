@@ -97,6 +97,25 @@ def test_fewer_rows_than_tokens_and_none(dev):
     _check(dev, past, new, table, free, count, 16, 0)
 
 
+def test_empty_stack(dev):
+    past, new = np.array([3, 16, 0]), np.array([1, 1, 0])
+    table = np.array([[5, -7], [6, -7], [-7, -7]], np.int32)
+    _check(dev, past, new, table, np.zeros(0, np.int32), 0, 16, 4)
+
+
+@pytest.mark.parametrize("num_rows", [8, 20001])
+def test_absurd_lengths_are_refused_in_bounds(dev, num_rows):
+    most = 2 ** 31 - 1
+    got = _run(dev, [0, 5, most, 1], [most, most, most, 1],
+               np.array([[0, 1], [2, 3], [4, 5], [6, 7]], np.int32), [8, 9], 2, 16, num_rows)
+    assert _capi.device_status(dev) == _capi.DEV_NO_PAGES
+    assert got["kv_lens"].tolist()[:3] == [0, 5, most]
+    assert got["cu_tokens"].tolist() == [0, most, most, most, most]
+    assert got["seq_ids"].tolist() == [0] * num_rows
+    assert got["slot_rows"].tolist() == [-1] * num_rows
+    assert got["free_count"].tolist() == [2]
+
+
 def test_all_leave_and_all_idle(dev):
     past, new, table, free, count = _case(13, 20, 16, 8, 100, 3, 4)
     _check(dev, past, np.full_like(new, -1), table, free, count, 16, 4)
