@@ -203,15 +203,16 @@ struct Sampler {
     const u64 w = weight_fixed(d * scale, s.table);
     return f >= least_logit ? w : 0;  // -inf is below it
   }
-  // Place on the bins' scale; bin b holds the places from b to b + 1 (with one bin
-  // for all, the places may be NaN: they count as its own).
-  __device__ __forceinline__ float place(float f) const { return (top - f) * bin_scale; }
+  // Place on the bins' scale, 0 .. inf; bin b holds the places from b to b + 1, the
+  // last bin all beyond.  (inf - inf and 0 * inf, of the largest logits: place 0.)
+  __device__ __forceinline__ float place(float f) const {
+    return fmaxf((top - f) * bin_scale, 0.f);
+  }
   __device__ __forceinline__ static bool between(float x, int b0, int b1) {  // bins b0 .. b1
-    return !(x < static_cast<float>(b0)) &&
-           (!(x >= static_cast<float>(b1 + 1)) || b1 == kSampBins - 1);
+    return x >= static_cast<float>(b0) && (x < static_cast<float>(b1 + 1) || b1 == kSampBins - 1);
   }
   __device__ __forceinline__ int bin(float f) const {
-    return min(kSampBins - 1, static_cast<int>((top - f) * bin_scale));  // f <= top; NaN: 0
+    return min(kSampBins - 1, static_cast<int>(place(f)));
   }
   __device__ __forceinline__ uint4 raw(int vec) const {
     const uint4* p = reinterpret_cast<const uint4*>(slice) + vec;

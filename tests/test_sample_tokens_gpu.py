@@ -202,6 +202,17 @@ def test_few_heavy_candidates_with_gaps(dev):
     _check(dev, x.to(dev), torch.rand(40, generator=g).tolist(), top_p=[min(q, 0.9999) for q in p])
 
 
+def test_infinities_and_a_large_k(dev):
+    """k reaches far beyond the infinite logits, into the last bin of all."""
+    x, u = _logits(4, 30000, 9, torch.float32)
+    x[0, 5::1000] = float("inf")
+    x[1, 100] = float("inf")
+    x[2, ::2] = float("inf")
+    k = [5000, 20000, 20000, 5000]
+    _check(dev, x.to(dev), u, top_k=k)
+    _check(dev, x.to(dev), u, top_k=k, top_p=[0.5, 0.9, 0.999, 0.9], temp=[1.0, 2.0, 0.1, 50.0])
+
+
 def test_wrapper_refusals(dev):
     x, u = torch.zeros(2, 8, device=dev), torch.zeros(2, device=dev)
     for bad in (lambda: _capi.sample_tokens(x.t(), u), lambda: _capi.sample_tokens(x, u[:1]),
