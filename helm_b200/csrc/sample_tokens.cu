@@ -20,7 +20,8 @@
 // memory.  With at least as many rows as SMs one CTA does a row, reading it from
 // L2 once per pass: no cluster barriers, and two rows share an SM, one computing
 // while the other waits (256 x 151936 bf16: top-k 144 -> 94 us, no filter 127 ->
-// 93).  Bound by instructions: some 30 per logit for its weight, 10 for a bin.
+// 93).  Bound by instructions: some 30 per logit for its weight, 10 for a bin; a
+// long bf16 row looks its weights up in a table of its possible values instead.
 //
 // A filter needs its last kept candidate.  A histogram of counts over 2048 equal
 // steps of the logit (equal steps spread a bell-shaped row over the bins; digits
@@ -41,6 +42,7 @@
 #include <cooperative_groups.h>
 
 #include <cstddef>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -59,6 +61,11 @@ constexpr int kSampMaxVocab = 1 << 18;       // 2^18 weights of 2^44 stay below 
 constexpr int kSampSliceBytes = 160 * 1024;  // most logits a CTA can hold
 constexpr int kSampSliceGoal = 80 * 1024;    // two CTAs an SM: one loads while the other computes
 constexpr int kSampMaxCluster = 8;
+// Table of weights (bf16): sixteen binades of magnitudes of either sign, and an
+// entry for what lies beyond.
+constexpr int kSampLutSide = 2048 + 1;
+constexpr int kSampLutBytes = 2 * kSampLutSide * 8;
+constexpr int kSampLutLogits = 65536;  // of a CTA, from which the table pays
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -72,6 +79,7 @@ struct SampleArgs {
   int64_t* ids;
   float* logprobs;
   int vocab, slice;  // logits of a row and of a CTA's slice
+  int tabled;        // room was given for the table of weights
 };
 
 // 2^(j/64), j = 0 .. 63, rounded to nearest
@@ -188,6 +196,9 @@ struct Sampler {
   double inv_temp, scale;  // z = (l - l_max) inv_temp, y = (l - l_max) scale
   float bin_scale;
   float least_logit;  // below it weights round to 0
+  u64* lut;           // weights by bf16 code, once `tabled`
+  int lut_base;       // magnitude code of its first entry
+  bool tabled = false;
 
   __device__ Sampler(const SampleArgs& a_, SampleShared& s_, const T* sl)
       : a(a_), s(s_), slice(sl), cluster(cg::this_cluster()) {
@@ -202,6 +213,33 @@ struct Sampler {
     const double d = static_cast<double>(fminf(f, 3.402823466e38f)) - top_finite;
     const u64 w = weight_fixed(d * scale, s.table);
     return f >= least_logit ? w : 0;  // -inf is below it
+  }
+  // weight() of a logit, from the table where there is one: a row has a few
+  // thousand bf16 values at most, and looking one up takes a third of the
+  // instructions.  Magnitudes below the table's are computed; those above are of
+  // logits too small to weigh, or +inf.
+  __device__ __forceinline__ u64 weight_of(float f) const {
+    if (!kResident && std::is_same<T, __nv_bfloat16>::value && tabled) {
+      const uint32_t u = __float_as_uint(f);
+      const int d = min(static_cast<int>((u & 0x7fffffffu) >> 16) - lut_base, kSampLutSide - 1);
+      if (d >= 0) return lut[d + (u >> 31 ? kSampLutSide : 0)];
+    }
+    return weight(f);
+  }
+  // smallest: the row's smallest finite logit
+  __device__ void build_table(float smallest) {
+    auto mag = [](float f) { return static_cast<int>((__float_as_uint(f) & 0x7fffffffu) >> 16); };
+    const int most = max(mag(static_cast<float>(top_finite)), mag(fmaxf(least_logit, smallest)));
+    lut_base = max(0, most + 2 - kSampLutSide);
+    for (int i = threadIdx.x; i < 2 * kSampLutSide; i += kSampThreads) {
+      const bool neg = i >= kSampLutSide;
+      const int d = neg ? i - kSampLutSide : i;
+      const float f = d < kSampLutSide - 1 ? __uint_as_float(static_cast<uint32_t>(lut_base + d) << 16)
+                                           : INFINITY;
+      lut[i] = weight(neg ? -f : f);
+    }
+    tabled = true;
+    __syncthreads();
   }
   // Place on the bins' scale, 0 .. inf; bin b holds the places from b to b + 1, the
   // last bin all beyond.  (inf - inf and 0 * inf, of the largest logits: place 0.)
@@ -346,7 +384,7 @@ struct Sampler {
       each(threadIdx.x, vecs, kSampThreads, [&](float f, int i) {
         if (f > -INFINITY && order_of(f, base + i) >= mid) {
           ++c;
-          m += weight(f);
+          m += weight_of(f);
         }
       });
       cluster_sum(c, m);
@@ -360,7 +398,7 @@ struct Sampler {
     }
     if (!have) {  // nothing reaches it: everything is kept
       u64 c = 0, m = 0;
-      each(threadIdx.x, vecs, kSampThreads, [&](float f, int) { m += weight(f); });
+      each(threadIdx.x, vecs, kSampThreads, [&](float f, int) { m += weight_of(f); });
       cluster_sum(c, m);
       at_lo = m;
     }
@@ -501,7 +539,7 @@ struct Sampler {
     const int s1 = seg_begin(warp + 1);
     SampleShared* home = cluster.map_shared_rank(&s, 0);
     each(seg_begin(warp) + lane, s1, 32, [&](float f, int i) {
-      const u64 w = weight(f);
+      const u64 w = weight_of(f);
       const float at_f = place(f);
       const bool over = at_f < static_cast<float>(lo);
       total += w;
@@ -660,6 +698,12 @@ struct Sampler {
         mp > 0.f ? min(u64(1) << 44, static_cast<u64>(ceil(static_cast<double>(mp) * 17592186044416.0)))
                  : 0;
 
+    const bool small_k = use_k && k <= ranks * (kSampThreads / 4);
+    // (greedy rows and those of a small k seldom weigh all logits)
+    if (!kResident && std::is_same<T, __nv_bfloat16>::value && a.tabled &&
+        (a.logprobs != nullptr || !(greedy || small_k)))
+      build_table(mn);
+
     // ---- where the filters cut -------------------------------------------------
     const int s0 = seg_begin(warp), s1 = seg_begin(warp + 1);
     u64 row_total = 0, above = 0;
@@ -673,7 +717,7 @@ struct Sampler {
       const float from = upto < kSampBins - 1 && low > -3.402823466e38f ? low : -3.402823466e38f;
       if (a.logprobs != nullptr || !use_k) {
         each(s0 + lane, s1, 32, [&](float f, int i) {
-          row_total += weight(f);
+          row_total += weight_of(f);
           if (f >= from) push(home, f, i);
         });
       } else {
@@ -693,7 +737,7 @@ struct Sampler {
       if (rank == 0) finish_few(row, k, use_k, p, use_p, least, u32, row_total);
       return true;  // rank 0 touches no other CTA's memory from here on
     };
-    if (use_k && k <= ranks * (kSampThreads / 4)) {
+    if (small_k) {
       if (try_few(bound_k(own_max, k))) return;
       // more than the list holds: start over with all logits
       for (int i = threadIdx.x; i < kSampBins; i += kSampThreads) s.hist[i] = 0;
@@ -713,13 +757,13 @@ struct Sampler {
     bool known = true;   // warp_kept is right
     if (greedy) {
       if (a.logprobs != nullptr)
-        each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight(f); });
+        each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight_of(f); });
       each(s0 + lane, s1, 32, [&](float f, int) { warp_kept += f == top ? 1 : 0; });
       warp_kept = warp_reduce(warp_kept, AddOp());
       if (a.logprobs != nullptr) cluster_sum(row_total, above);
     } else if (!use_k && !use_p) {
       each(s0 + lane, s1, 32, [&](float f, int) {
-        const u64 w = weight(f);
+        const u64 w = weight_of(f);
         row_total += w;
         warp_kept += w >= least ? w : 0;
       });
@@ -797,7 +841,7 @@ struct Sampler {
     auto keep = [&](float f, int i) -> u64 {
       if (greedy) return f == top ? 1 : 0;
       if (last != 0 && order_of(f, base + i) < last) return 0;
-      const u64 w = weight(f);
+      const u64 w = weight_of(f);
       return w >= least ? w : 0;
     };
     if (!known) {
@@ -967,6 +1011,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_tokens_kernel(const Sa
   SampleShared& s = *reinterpret_cast<SampleShared*>(s_raw);
   T* slice = reinterpret_cast<T*>(s_raw + (sizeof(SampleShared) + 15) / 16 * 16);
   Sampler<T, kResident> job(a, s, slice);
+  job.lut = reinterpret_cast<u64*>(slice);  // where the row is not resident
   constexpr int kVec = 16 / sizeof(T);
   const int row = blockIdx.x / job.ranks;
   job.base = min(a.vocab, job.rank * a.slice);
@@ -1019,20 +1064,27 @@ cudaError_t launch_sample(SampleArgs a, int batch, int ctas, cudaStream_t stream
   static unsigned long long configured = 0;  // one bit per device
   constexpr int kFixed = (sizeof(SampleShared) + 15) / 16 * 16;
   static_assert(kFixed + kSampSliceBytes <= 227 * 1024, "");
+  static_assert(2 * (kFixed + kSampLutBytes) <= 226 * 1024, "two CTAs an SM");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (kResident && (dev >= 64 || !(configured & (1ull << dev)))) {
+  if (dev >= 64 || !(configured & (1ull << dev))) {
     e = cudaFuncSetAttribute(sample_tokens_kernel<T, kResident>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kSampSliceBytes);
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kFixed + (kResident ? kSampSliceBytes : kSampLutBytes));
     if (e != cudaSuccess) return e;
     if (dev < 64) configured |= 1ull << dev;
   }
   a.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
+  // The table of weights costs 4098 of them: slower with the slices of a cluster
+  // (64 x 151936 in slices of 19k: 66.8 -> 69.8 us), faster with whole rows (256 x
+  // 151936, no filter: 93 -> 75, top-p 220 -> 200).
+  a.tabled = !kResident && std::is_same<T, __nv_bfloat16>::value && a.vocab >= kSampLutLogits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));
   cfg.blockDim = dim3(kSampThreads);
-  cfg.dynamicSmemBytes = kFixed + (kResident ? static_cast<size_t>(a.slice) * sizeof(T) : 0);
+  cfg.dynamicSmemBytes = kFixed + (kResident ? static_cast<size_t>(a.slice) * sizeof(T) : 0) +
+                         (a.tabled ? kSampLutBytes : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1077,7 +1129,7 @@ extern "C" int helm_sample_tokens(const void* logits, int64_t row_stride, int dt
   if (batch == 0) return HELM_OK;
   if (vocab > kSampMaxVocab || batch > (1 << 24)) return HELM_ERR_UNSUPPORTED;
   const SampleArgs a = {logits, row_stride, uniforms, temperature, top_k, top_p,
-                        min_p,  ids,        logprobs, vocab,       0};
+                        min_p,  ids,        logprobs, vocab,       0,           0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (dtype) {

@@ -213,6 +213,43 @@ def test_infinities_and_a_large_k(dev):
     _check(dev, x.to(dev), u, top_k=k, top_p=[0.5, 0.9, 0.999, 0.9], temp=[1.0, 2.0, 0.1, 50.0])
 
 
+def test_long_bf16_rows_of_every_kind(dev):
+    """As many rows as SMs: weights come from the table of bf16 values, whatever the row holds."""
+    b, v = 160, 65544
+    x, u = _logits(b, v, v, torch.bfloat16)
+    for i in range(b):
+        row, kind = x[i], i % 10
+        if kind == 1:
+            row[::3] = float("-inf")
+        elif kind == 2:
+            row[::2] = 0.0
+            row[1::8] = -0.0
+        elif kind == 3:
+            row *= 2.0 ** -20                 # all weights nearly alike
+        elif kind == 4:
+            row -= 300                        # all negative, coarse steps
+        elif kind == 5:
+            row *= 1e4
+            row[7] = float("nan")
+        elif kind == 6:
+            row[5::1000] = float("inf")
+        elif kind == 7:
+            row[:] = row[0]
+        elif kind == 8:
+            row[:-3] = float("-inf")
+            row[-2] = torch.finfo(torch.bfloat16).min
+        elif kind == 9:
+            row[::5] *= 1e-30                 # far below the table's magnitudes
+    x = x.to(dev)
+    i = np.arange(b)
+    temp = np.where(i % 7 == 6, 0.0, np.where(i % 20 == 15, 3e4, 0.4 + i / 100))
+    p = np.where(i % 3 == 1, 0.2 + i / 250, 1.0)
+    k = np.where(i % 4 == 2, 1 + 37 * i, 0)
+    m = np.where(i % 5 == 3, 0.01, 0.0)
+    _check(dev, x, u, temp=temp, top_k=k, top_p=p, min_p=m)
+    _check(dev, x, u, temp=temp, top_p=p, want_logp=False)
+
+
 def test_wrapper_refusals(dev):
     x, u = torch.zeros(2, 8, device=dev), torch.zeros(2, device=dev)
     for bad in (lambda: _capi.sample_tokens(x.t(), u), lambda: _capi.sample_tokens(x, u[:1]),
