@@ -37,7 +37,9 @@
 // For a small k the histogram need not see every logit: the threads' own largest
 // ones bound the k-th from below (k of them at or above a bin are k candidates),
 // and the candidates from that bin up are few.
-// Whatever neither can decide (more than 1024 equal logits at the cut, say) is
+// A long bf16 row counts its logits by value instead (by_value), which says exactly
+// where the filters cut.
+// Whatever these cannot decide (more than 1024 equal logits at the cut, say) is
 // bisected over the order of candidates, pass by pass.
 #include <cooperative_groups.h>
 
@@ -64,7 +66,7 @@ constexpr int kSampMaxCluster = 8;
 // Table of weights (bf16): sixteen binades of magnitudes of either sign, and an
 // entry for what lies beyond.
 constexpr int kSampLutSide = 2048 + 1;
-constexpr int kSampLutBytes = 2 * kSampLutSide * 8;
+constexpr int kSampLutBytes = 2 * kSampLutSide * (8 + 4);  // weights and counts
 constexpr int kSampLutLogits = 65536;  // of a CTA, from which the table pays
 typedef unsigned long long u64;
 
@@ -220,11 +222,15 @@ struct Sampler {
   // logits too small to weigh, or +inf.
   __device__ __forceinline__ u64 weight_of(float f) const {
     if (!kResident && std::is_same<T, __nv_bfloat16>::value && tabled) {
-      const uint32_t u = __float_as_uint(f);
-      const int d = min(static_cast<int>((u & 0x7fffffffu) >> 16) - lut_base, kSampLutSide - 1);
-      if (d >= 0) return lut[d + (u >> 31 ? kSampLutSide : 0)];
+      const int at = lut_entry(f);
+      if (at >= 0) return lut[at];
     }
     return weight(f);
+  }
+  __device__ __forceinline__ int lut_entry(float f) const {  // -1: below the table
+    const uint32_t u = __float_as_uint(f);
+    const int d = min(static_cast<int>((u & 0x7fffffffu) >> 16) - lut_base, kSampLutSide - 1);
+    return d < 0 ? -1 : d + (u >> 31 ? kSampLutSide : 0);
   }
   // smallest: the row's smallest finite logit
   __device__ void build_table(float smallest) {
@@ -556,6 +562,172 @@ struct Sampler {
     });
   }
 
+  // The filters of a row whose values have a table (one CTA): the logits are counted
+  // by value, and counts times weights, taken in the order of the values, say
+  // exactly in which value each filter ends and how many of its candidates, in
+  // index order, are kept.  One more pass sums what is kept and finds the last of
+  // those.  (256 x 151936, top-p: 210 us without it, 138 with.)  False where a filter
+  // ends among the values below the table, which are counted as one.
+  static constexpr int kLutPos = 2 * kSampLutSide + 1;  // positive, below the table, negative
+  static constexpr int kLutPer = (kLutPos + kSampThreads - 1) / kSampThreads;
+  __device__ bool by_value(int k, bool use_k, float p, bool use_p, u64 least, u64& total, u64& last,
+                           u64& warp_kept, bool& known) {
+    uint32_t* counts = reinterpret_cast<uint32_t*>(lut + 2 * kSampLutSide);
+    for (int i = threadIdx.x; i < 2 * kSampLutSide; i += kSampThreads) counts[i] = 0;
+    if (threadIdx.x == 0) {
+      s.bin_k = s.bin_p = -1;
+      s.in_k = 0;      // candidates below the table
+      s.win_over = 0;  // and their weight
+    }
+    __syncthreads();
+    uint32_t tiny_n = 0;
+    u64 tiny_w = 0;
+    each(threadIdx.x, vecs, kSampThreads, [&](float f, int) {
+      if (!(f > -INFINITY)) return;
+      const int at = lut_entry(f + 0.f);  // -0 with +0
+      if (at >= 0) {
+        atomicAdd(counts + at, 1u);
+      } else {
+        ++tiny_n;
+        tiny_w += weight(f);
+      }
+    });
+    if (__any_sync(0xffffffffu, tiny_n != 0)) {
+      tiny_n = warp_reduce(tiny_n, AddOp());
+      tiny_w = warp_reduce(tiny_w, AddOp());
+      if (lane == 0) {
+        atomicAdd(&s.in_k, tiny_n);
+        atomicAdd(&s.win_over, tiny_w);
+      }
+    }
+    __syncthreads();
+    // places in descending order of value; this thread's are first .. first + kLutPer - 1
+    const int first = threadIdx.x * kLutPer;
+    auto at_place = [&](int pos, uint32_t& c, u64& w) {  // candidates and weight of each; its mass
+      c = 0;
+      w = 0;
+      if (pos >= kLutPos) return u64(0);
+      if (pos == kSampLutSide) {
+        c = s.in_k;
+        return s.win_over;
+      }
+      const int at = lut_of(pos);
+      c = counts[at];
+      w = lut[at];
+      return c * w;
+    };
+    uint32_t c, n = 0, all_n;
+    u64 w, m = 0;
+    for (int i = 0; i < kLutPer; ++i) {
+      m += at_place(first + i, c, w);
+      n += c;
+    }
+    const uint32_t n0 = block_scan(n, reinterpret_cast<uint32_t*>(s.warp_a), all_n);
+    const u64 m0 = block_scan(m, s.warp_a, total);
+    const uint32_t uk = static_cast<uint32_t>(k);
+    if (use_k && n0 < uk && n0 + n >= uk) {
+      u64 mass = m0;
+      for (int i = 0, before = n0; i < kLutPer; ++i) {
+        const u64 here = at_place(first + i, c, w);
+        if (before < k && before + static_cast<int>(c) >= k) {
+          s.bin_k = first + i;
+          s.upto_k = uk - before;
+          s.last_mass = mass + s.upto_k * w;
+        }
+        before += c;
+        mass += here;
+      }
+    }
+    __syncthreads();
+    int cut = -1;
+    uint32_t need = 0;
+    u64 of = total;
+    if (use_k && s.bin_k >= 0) {
+      cut = s.bin_k;
+      need = s.upto_k;
+      of = s.last_mass;
+      if (cut == kSampLutSide) return false;
+    }
+    if (use_p) {
+      const u64 target = top_p_target(p, of);
+      if (m0 < target && m0 + m >= target) {
+        u64 mass = m0;
+        for (int i = 0; i < kLutPer; ++i) {
+          const u64 here = at_place(first + i, c, w);
+          if (mass < target && mass + here >= target) {
+            s.bin_p = first + i;
+            s.upto_p = w != 0 ? static_cast<uint32_t>((target - mass + w - 1) / w) : 0;
+          }
+          mass += here;
+        }
+      }
+      __syncthreads();
+      cut = s.bin_p;
+      need = s.upto_p;
+      if (cut < 0 || cut == kSampLutSide) return false;
+    }
+    last = 0;
+    known = false;
+    const int at = cut < 0 ? 0 : lut_of(cut);
+    const u64 w_cut = cut < 0 ? 0 : lut[at];
+    if (w_cut == 0) return true;  // whatever has a weight is kept
+    const bool neg = at >= kSampLutSide;
+    const int d = neg ? at - kSampLutSide : at;
+    const float mag = d == kSampLutSide - 1
+                          ? INFINITY
+                          : __uint_as_float(static_cast<uint32_t>(lut_base + d) << 16);
+    const float v = neg ? -mag : mag;
+    uint32_t equal = 0;
+    u64 above = 0;
+    each(seg_begin(warp) + lane, seg_begin(warp + 1), 32, [&](float f, int) {
+      if (f > v) {
+        const u64 x = weight_of(f);
+        above += x >= least ? x : 0;
+      }
+      equal += f == v ? 1 : 0;
+    });
+    above = warp_reduce(above, AddOp());
+    equal = warp_reduce(equal, AddOp());
+    if (lane == 0) s.warp_b[warp] = equal;
+    __syncthreads();
+    const uint32_t mine = lane < kSampWarps ? static_cast<uint32_t>(s.warp_b[lane]) : 0;
+    uint32_t inc = mine;
+#pragma unroll
+    for (int off = 1; off < kSampWarps; off <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += x;
+    }
+    const uint32_t ex = inc - mine, ahead = __shfl_sync(0xffffffffu, ex, warp);
+    const uint32_t kept = min(equal, need > ahead ? need - ahead : 0u);
+    warp_kept = above + (w_cut >= least ? kept * w_cut : 0);
+    known = true;
+    if (need >= counts[at]) {
+      last = static_cast<u64>(order_key(v)) << 32;
+      return true;
+    }
+    // the need-th candidate of this value: the warp's run that holds it, again
+    const unsigned hit = __ballot_sync(0xffffffffu, lane < kSampWarps && ex < need && inc >= need);
+    const int run = max(0, __ffs(hit) - 1);
+    const uint32_t rest = need - __shfl_sync(0xffffffffu, ex, run);
+    const int v0 = seg_begin(run), v1 = seg_begin(run + 1);
+    const int per = (v1 - v0 + kSampThreads - 1) / kSampThreads;
+    const int t0 = min(v1, v0 + static_cast<int>(threadIdx.x) * per), t1 = min(v1, t0 + per);
+    uint32_t here = 0, sum;
+    each(t0, t1, 1, [&](float f, int) { here += f == v ? 1 : 0; });
+    uint32_t seen = block_scan(here, reinterpret_cast<uint32_t*>(s.warp_a), sum);
+    if (seen < rest && seen + here >= rest) {
+      each(t0, t1, 1, [&](float f, int i) {
+        if (f == v && ++seen == rest) s.last = order_of(f, base + i);
+      });
+    }
+    __syncthreads();
+    last = s.last;
+    return true;
+  }
+  __device__ __forceinline__ static int lut_of(int pos) {  // table entry of a place
+    return pos < kSampLutSide ? kSampLutSide - 1 - pos : pos - 1;
+  }
+
   // After weigh() and a cluster barrier: the bin of the window in which the
   // weight from the top reaches target, -1 if none; over: the weight above it.
   __device__ int window_find(int lo, u64 above, u64 target, u64& over) {
@@ -743,7 +915,15 @@ struct Sampler {
       for (int i = threadIdx.x; i < kSampBins; i += kSampThreads) s.hist[i] = 0;
       __syncthreads();
     }
-    if (use_k || use_p) {
+    u64 last = 0;        // every candidate from this order on is kept
+    u64 warp_kept = 0;   // of this warp's run of vectors
+    bool known = true;   // warp_kept is right
+    bool counted = false;
+    if (!kResident && std::is_same<T, __nv_bfloat16>::value && tabled && (use_k || use_p)) {
+      counted = by_value(k, use_k, p, use_p, least, row_total, last, warp_kept, known);
+      if (!counted) row_total = 0;
+    }
+    if (!counted && (use_k || use_p)) {
       histogram(k, use_k, p, use_p);
       // (top-p alone: the window and the margin, whichever reaches further)
       if ((use_k ? s.upto_k : max(s.upto_w, s.upto_f)) <= kSampList &&
@@ -752,10 +932,9 @@ struct Sampler {
     }
 
     // ---- many candidates, or no filter ------------------------------------------
-    u64 last = 0;        // every candidate from this order on is kept
-    u64 warp_kept = 0;   // of this warp's run of vectors
-    bool known = true;   // warp_kept is right
-    if (greedy) {
+    if (counted) {
+      // (by_value has what the draw needs)
+    } else if (greedy) {
       if (a.logprobs != nullptr)
         each(s0 + lane, s1, 32, [&](float f, int) { row_total += weight_of(f); });
       each(s0 + lane, s1, 32, [&](float f, int) { warp_kept += f == top ? 1 : 0; });
@@ -1078,7 +1257,7 @@ cudaError_t launch_sample(SampleArgs a, int batch, int ctas, cudaStream_t stream
   a.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
   // The table of weights costs 4098 of them: slower with the slices of a cluster
   // (64 x 151936 in slices of 19k: 66.8 -> 69.8 us), faster with whole rows (256 x
-  // 151936, no filter: 93 -> 75, top-p 220 -> 200).
+  // 151936, no filter: 93 -> 81, top-k 95 -> 79, top-p with by_value 220 -> 138).
   a.tabled = !kResident && std::is_same<T, __nv_bfloat16>::value && a.vocab >= kSampLutLogits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));

@@ -250,6 +250,34 @@ def test_long_bf16_rows_of_every_kind(dev):
     _check(dev, x, u, temp=temp, top_p=p, want_logp=False)
 
 
+def test_long_bf16_rows_cut_at_every_place(dev):
+    """Filters that end among values far below the largest, at zeros of both signs, at
+    the last candidate, among candidates without weight, and within many equal ones."""
+    b, v = 160, 65536
+    x, u = _logits(b, v, 77, torch.bfloat16)
+    g = torch.Generator().manual_seed(78)
+    for i in range(b):
+        row, kind = x[i], i % 5
+        if kind == 1:
+            row *= 1e-30
+            row[i] = 2.0
+        elif kind == 2:
+            row[torch.randperm(v, generator=g)[:50000]] = 0.0
+            row[::7] = -0.0
+            row.clamp_(max=0.0)
+        elif kind == 3:
+            row[:] = torch.randint(0, 3, (v,), generator=g).to(torch.bfloat16)
+        elif kind == 4:
+            row[100:] -= 1000
+            row[v // 2:] = float("-inf")
+    x = x.to(dev)
+    i = np.arange(b)
+    p = 0.03 + 0.96 * (i * 37 % b) / b
+    k = np.where(i % 3 == 0, 1 + i * 400, np.where(i % 3 == 1, v - 1 - i, 0))
+    _check(dev, x, u, top_p=p)
+    _check(dev, x, u, top_k=k, top_p=np.where(i % 4 == 1, p, 1.0))
+
+
 def test_wrapper_refusals(dev):
     x, u = torch.zeros(2, 8, device=dev), torch.zeros(2, device=dev)
     for bad in (lambda: _capi.sample_tokens(x.t(), u), lambda: _capi.sample_tokens(x, u[:1]),
