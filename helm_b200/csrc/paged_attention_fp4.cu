@@ -27,7 +27,8 @@
 //     once for both.
 // q is scaled per head by a power of two into fp16's range.  P is rounded to
 // fp16 (half a step: 2^-11) where O is bf16 (2^-8); where O is fp16 itself it
-// is carried as the sum of two fp16 numbers.  The sum l and all state are fp32.
+// is carried as the sum of two fp16 numbers, the second in a product's idle
+// columns where there are enough.  The sum l and all state are fp32.
 //
 // All units of all (sequence, KV head) pairs lie in one flattened order, cut into
 // equal contiguous ranges, one per warp (paged_attention.cu's split).  A warp's
@@ -254,10 +255,14 @@ __device__ __forceinline__ Fp4Span fp4_span(const DecodeFp4Args& a, const int* s
   return ps;
 }
 
-template <typename T, int D, int NT, bool kPlain>
+// kFold (fp16, at most four heads a KV head): heads 0 .. 3 stand again in columns
+// 4 .. 7 of the products, whose P is the low half; so the second product of a
+// split P costs nothing.
+template <typename T, int D, int NT, bool kPlain, bool kFold>
 struct Fp4Worker {
   static constexpr int KS = D / 16;
-  static constexpr bool kSplitP = std::is_same<T, __half>::value;
+  static constexpr bool kSplitP = std::is_same<T, __half>::value && !kFold;
+  static_assert(!kFold || (NT == 1 && std::is_same<T, __half>::value), "");
   using L = Fp4Tile<D>;
   float m[NT][2];       // running maximum (units: see DecodeFp4Args), it may lag by 2^8
   float l[NT][2];
@@ -315,7 +320,7 @@ struct Fp4Worker {
     const T* qb = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.q_sb;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int hg = nt * 8 + r;
+      const int hg = kFold ? r & 3 : nt * 8 + r;
       const bool ok = hg < a.group;
       const T* qh = qb + static_cast<int64_t>(h * a.group + (ok ? hg : 0)) * a.q_sh;
       float amax = 0.f;
@@ -367,6 +372,12 @@ struct Fp4Worker {
   __device__ __forceinline__ void flush(const DecodeFp4Args& a, bool alone, int v, int lane) {
     const int r = lane >> 2, c = lane & 3;
     const int p = cur_b * a.hkv + cur_h;
+    if (kFold) {  // columns 4 .. 7 (lanes c + 2) join 0 .. 3
+#pragma unroll
+      for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][mt][e] += __shfl_xor_sync(0xffffffffu, o[0][mt][e], 2);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -617,13 +628,13 @@ struct Fp4Worker {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t hi = MmaOp<__half>::pack(p[2 * i], p[2 * i + 1]);
-          pb[ti][nt][i] = movmatrix_trans(hi);
-          pl[ti][nt][i] = 0;
-          if (kSplitP) {
+          uint32_t lo = 0;
+          if (kSplitP || kFold) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            pl[ti][nt][i] = movmatrix_trans(
-                MmaOp<__half>::pack(p[2 * i] - f.x, p[2 * i + 1] - f.y));
+            lo = MmaOp<__half>::pack(p[2 * i] - f.x, p[2 * i + 1] - f.y);
           }
+          pb[ti][nt][i] = movmatrix_trans(kFold && (lane & 2) ? lo : hi);
+          pl[ti][nt][i] = kSplitP ? movmatrix_trans(lo) : 0;
         }
       }
     values(base, pb[0], pl[0], keep01[0], keep23[0]);
@@ -631,7 +642,7 @@ struct Fp4Worker {
   }
 };
 
-template <typename T, int D, int NT, bool kPlain>
+template <typename T, int D, int NT, bool kPlain, bool kFold>
 __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
     paged_decode_fp4_kernel(const DecodeFp4Args a) {
   using S = Fp4Shape<D, NT>;
@@ -712,7 +723,7 @@ __global__ void __launch_bounds__(Fp4Shape<D, NT>::kThreads, 1)
     if (a.lse != nullptr && threadIdx.x < a.group)
       a.lse[static_cast<int64_t>(b) * a.hq + h * a.group + threadIdx.x] = -INFINITY;
   }
-  Fp4Worker<T, D, NT, kPlain> st;
+  Fp4Worker<T, D, NT, kPlain, kFold> st;
   st.lane_offsets(lane);
   bool ok = true;
   int stage = 0, parity = 0;
@@ -890,7 +901,7 @@ __global__ void __launch_bounds__(kFp4MergeThreads) merge_fp4_kernel(const Decod
 }
 
 // ----------------------------------------------------------------- host side --
-template <typename T, int D, int NT, bool kPlain>
+template <typename T, int D, int NT, bool kPlain, bool kFold = false>
 cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_units, cudaStream_t stream) {
   using S = Fp4Shape<D, NT>;
   static unsigned long long configured = 0;  // one bit per device
@@ -898,7 +909,7 @@ cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_units, cudaStream_t s
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(configured & (1ull << dev))) {
-    e = cudaFuncSetAttribute(paged_decode_fp4_kernel<T, D, NT, kPlain>,
+    e = cudaFuncSetAttribute(paged_decode_fp4_kernel<T, D, NT, kPlain, kFold>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(S::smem_bytes(kMaxBatch)));
     if (e != cudaSuccess) return e;
@@ -921,7 +932,7 @@ cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_units, cudaStream_t s
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(a.warps * 32);
   cfg.dynamicSmemBytes = S::smem_bytes(a.batch);
-  e = cudaLaunchKernelEx(&cfg, paged_decode_fp4_kernel<T, D, NT, kPlain>, a);
+  e = cudaLaunchKernelEx(&cfg, paged_decode_fp4_kernel<T, D, NT, kPlain, kFold>, a);
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.hkv), static_cast<unsigned>(a.group),
                      D / 4 / kFp4MergeCols);
@@ -933,6 +944,10 @@ cudaError_t launch_decode_fp4(DecodeFp4Args a, int64_t max_units, cudaStream_t s
 template <typename T, int D>
 cudaError_t dispatch_decode_fp4_nt(const DecodeFp4Args& a, bool plain, int64_t units,
                                    cudaStream_t s) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  if (kHalf && a.group <= 4)  // 16 x 2k tokens, one head a KV head: 50.4 us, two products 53.9
+    return plain ? launch_decode_fp4<T, D, 1, true, kHalf>(a, units, s)
+                 : launch_decode_fp4<T, D, 1, false, kHalf>(a, units, s);
   if (a.group <= 8)
     return plain ? launch_decode_fp4<T, D, 1, true>(a, units, s)
                  : launch_decode_fp4<T, D, 1, false>(a, units, s);

@@ -245,6 +245,10 @@ CASES = [
     ([200, 18], 32, 2, 256, 16, FP16, 0.0, 1.0, 1.0),
     ([4099], 5, 1, 128, 16, BF16, 0.0, 1.0, 1.0),            # one pair over many CTAs
     ([2500, 900, 31], 7, 1, 64, 16, BF16, 20.0, 1.0, 1.0),
+    ([4099, 5], 4, 1, 128, 16, FP16, 0.0, 1.0, 1.0),         # fp16, up to four heads a KV head
+    ([1500, 203, 0], 6, 2, 64, 16, FP16, 30.0, 1.0, 1.0),
+    ([310, 77], 4, 2, 256, 32, FP16, 0.0, 0.5, 2.0),
+    ([900, 33], 10, 2, 128, 16, FP16, 0.0, 1.0, 1.0),        # five
 ]
 
 
