@@ -482,23 +482,26 @@ struct Sampler {
       }
     }
     if (use_p) {
-      // weights at the bins' centres (fp32: an estimate); with top-k the first k
+      // weights at the bins' centres (an estimate); with top-k the first k.  In whole
+      // numbers, steps of 2^-40 and one at least: the threads' shares then tile the
+      // sum exactly, so one thread of the CTA holds the bin, and the same bin in
+      // every CTA of the cluster (fp32 running sums overlap by their rounding).
       const float step = bin_scale > 0.f ? static_cast<float>(inv_temp) / bin_scale : 0.f;
-      float m[kPer], sum = 0.f;
+      u64 m[kPer], sum = 0, all;
       before = ex;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const uint32_t count = use_k ? min(c[i], before < uk ? uk - before : 0u) : c[i];
-        m[i] = static_cast<float>(count) * (__expf(-(b0 + i + 0.5f) * step) + 1e-30f);
+        const float e = fmaxf(__expf(-(b0 + i + 0.5f) * step), 0.f);  // (NaN: 0)
+        m[i] = count * (static_cast<u64>(e * 0x1p40f) + 1);
         sum += m[i];
         before += c[i];
       }
-      float all;
-      float at = block_scan(sum, s.warp_min, all);
-      const float want = p * all;
+      u64 at = block_scan(sum, s.warp_a, all);
+      const u64 want = top_p_target(p, all);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        if (m[i] > 0.f && at < want && at + m[i] >= want) s.bin_p = b0 + i;
+        if (at < want && at + m[i] >= want) s.bin_p = b0 + i;
         at += m[i];
       }
     }
