@@ -333,7 +333,9 @@ class TPDecodeModel:
     def _step(self, forced: Optional[torch.Tensor] = None) -> None:
         """One decode step: the token in self.ids is appended at position
         lens and attended; self.ids becomes the greedy next token (or, when
-        `forced` [B, 1] is given, that token; the argmax stays in self.next)."""
+        `forced` [B, 1] is given, that token; the argmax stays in self.next).
+        Over 4-bit pages a sequence that is idle or leaves keeps its token unless
+        another is forced, and one that is refused a page keeps it in any case."""
         w, B, D, P = self.w, self.B, self.D, self.P
         h = self.h
         torch.index_select(w.embed, 0, self.ids.view(-1), out=h)
@@ -380,10 +382,15 @@ class TPDecodeModel:
         else:
             nxt = self._greedy()
         self.next = nxt.long().view(B, 1)
-        if self.fp4:   # a sequence that is idle keeps its token
-            self.next = torch.where(self.new_lens.view(B, 1) > 0, self.next, self.ids)
+        new = self.next if forced is None else forced.to(self.dev)
+        if self.fp4:
+            # a sequence that is idle keeps its token; one that was refused a page keeps
+            # it whatever is forced: the token has not been cached yet
+            took, asked = (lens1 > self.lens).view(B, 1), (self.new_lens > 0).view(B, 1)
+            self.next = torch.where(took, self.next, self.ids)
+            new = self.next if forced is None else torch.where(asked & ~took, self.ids, new)
         self.lens.copy_(lens1)
-        self.ids.copy_(self.next if forced is None else forced)
+        self.ids.copy_(new)
 
     def _greedy(self) -> torch.Tensor:
         """Greedy pick over the vocab shards: (max value, global index) per rank."""
