@@ -19,15 +19,17 @@
 //     tile's layout makes those reads conflict-free.
 //   * V fragments pair two tokens of one dim.  Nibbles of two token words are
 //     interleaved before widening (four logic ops per 16 values).
-//   * The running maximum moves only when a score exceeds it by 8 in log2
-//     units (then P <= 2^8, far inside fp16), so a unit normally costs one
-//     vote instead of a max reduction and a rescale of O.
+//   * P is taken against a reference that lies 2^11 below the running maximum and
+//     moves only when a P would exceed 2^15, fp16's last binade: a unit normally
+//     costs one vote instead of a max reduction and a rescale of O, and weights
+//     down to 2^-25 of the largest keep all of fp16's bits.
 //   * Work goes by UNITS of two tiles (32 tokens): their chains of LDS, cvt,
 //     mma and exp2 are independent, and waits, votes and bookkeeping are paid
 //     once for both.
 // q is scaled per head by a power of two into fp16's range.  P is rounded to
-// fp16 (half a step: 2^-11) where O is bf16 (2^-8); where O is fp16 itself it
-// is carried as the sum of two fp16 numbers, the second in a product's idle
+// fp16 where O is bf16 (half a step 2^-8): it is off by 2^-11 of itself, or by 2^-36
+// of the largest where that is more; where O is fp16 itself it is carried as the sum
+// of two fp16 numbers (2^-22, the same floor), the second in a product's idle
 // columns where there are enough.  The sum l and all state are fp32.
 //
 // All units of all (sequence, KV head) pairs lie in one flattened order, cut into
@@ -68,14 +70,17 @@ struct DecodeFp4Args {
   float score_scale; // softmax scale x K cache scale
   float softcap, softcap_inv;
   float v_scale;
-  // A state's maximum m is in log2 units in the plain form (no mask, no softcap,
+  // A state's reference m is in log2 units in the plain form (no mask, no softcap,
   // scale > 0), in natural units of the score otherwise (a mask of the type's
   // lowest value must not overflow):
-  float unit_log2;   // exp2 factor of a difference of maxima: 1 or log2(e)
+  float unit_log2;   // exp2 factor of a difference of references: 1 or log2(e)
   float unit_ln;     // natural units of m: ln 2 or 1
 };
 
 constexpr float kLowest = -3.402823466e38f;
+// log2 of the largest P, and of P at the maximum when the reference has just moved:
+// the maximum may rise by the difference before it moves again.
+constexpr float kMostP = 15.f, kTopP = 11.f;
 constexpr int kUnitTokens = 2 * kFp4TileTokens;
 constexpr int kFp4MaxWarps = 16;  // of a CTA (sizes the workspace)
 
@@ -264,7 +269,7 @@ struct Fp4Worker {
   static constexpr bool kSplitP = std::is_same<T, __half>::value && !kFold;
   static_assert(!kFold || (NT == 1 && std::is_same<T, __half>::value), "");
   using L = Fp4Tile<D>;
-  float m[NT][2];       // running maximum (units: see DecodeFp4Args), it may lag by 2^8
+  float m[NT][2];       // what P is taken against (units: see DecodeFp4Args)
   float l[NT][2];
   float o[NT][KS][4];
   uint32_t qf[NT][KS][2];
@@ -578,7 +583,7 @@ struct Fp4Worker {
             ((eB >> (8 * c)) & 1 ? 0x0000ffffu : 0u) | ((eB >> (8 * c + 4)) & 1 ? 0xffff0000u : 0u);
       }
     }
-    // exponents against the running maximum; it moves when one exceeds 8
+    // exponents against the reference; it moves when one exceeds kMostP
     float t[2][NT][4];
     auto exponents = [&]() {
       float hi = -1.f;
@@ -595,7 +600,7 @@ struct Fp4Worker {
           }
       return hi;
     };
-    if (__any_sync(0xffffffffu, exponents() > 8.f)) {
+    if (__any_sync(0xffffffffu, exponents() > kMostP)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -603,7 +608,7 @@ struct Fp4Worker {
           float mx = fmaxf(fmaxf(s[0][nt][j], s[0][nt][2 + j]), fmaxf(s[1][nt][j], s[1][nt][2 + j]));
           mx = warp_max_xor(mx, 4, 16);
           if (kPlain) mx *= cx[nt][j];
-          const float m_new = fmaxf(m[nt][j], mx);
+          const float m_new = fmaxf(m[nt][j], mx - (kPlain ? kTopP : kTopP * kLn2));
           const float alpha = exp2_fast((m[nt][j] - m_new) * (kPlain ? 1.f : kLog2e));
           m[nt][j] = m_new;
           l[nt][j] *= alpha;
