@@ -116,7 +116,7 @@ __device__ __forceinline__ float tanh_fast(float x) {
   const float small = fmaf(p * z, x, x);
   const float e = exp2_fast(fabsf(x) * (2.f * kLog2e));  // inf: 1
   const float large = copysignf(1.f - __fdividef(2.f, e + 1.f), x);
-  return z < 0.0625f ? small : (e < INFINITY ? large : copysignf(1.f, x));
+  return z < 0.0625f ? small : (e == INFINITY ? copysignf(1.f, x) : large);  // NaN stays NaN
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint64_t* bar) {

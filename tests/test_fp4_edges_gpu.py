@@ -74,3 +74,35 @@ def test_many_light_keys_beside_a_heavy_one(dev, dtype, hq, nats):
         assert (np.abs(got - want) <= tol).all(), np.abs((got - want) / tol).max()
         off = lse.double().cpu().numpy() - (6 * scale + np.log(w.sum()))
         assert (np.abs(off) <= l_err + 20 * 2.0 ** -22).all(), np.abs(off).max()
+
+
+@pytest.mark.parametrize("dtype,hq,d", [(BF16, 8, 128), (FP16, 4, 64), (BF16, 4, 256), (FP16, 24, 128)])
+def test_a_visible_nan_is_not_hidden_by_the_soft_cap(dev, dtype, hq, d):
+    g = torch.Generator().manual_seed(d + hq)
+    n, hkv, page = 90, 2, 16
+    k = torch.randn(n, hkv, d, generator=g).to(dtype)
+    v = torch.randn(n, hkv, d, generator=g).to(dtype)
+    q = torch.randn(1, hq, d, generator=g).to(dtype)
+    kw = dict(num_kv_heads=hkv, page_size=page, scale=0.1)
+
+    def run(k, q, cap):
+        pool, table, lens = _pool(dev, k, v, page)
+        lse = torch.empty(1, hq, device=dev)
+        out, _ = _capi.paged_decode_attention_fp4(q.to(dev), pool, table, lens, lse=lse, softcap=cap,
+                                                  **kw)
+        return out.cpu()[0], lse.cpu()[0]
+
+    for cap in (0.0, 30.0):
+        ref, ref_lse = run(k, q, cap)
+        bad_k = k.clone()
+        bad_k[37, 1, 5] = float("nan")       # its block of KV head 1
+        out, lse = run(bad_k, q, cap)
+        clean = slice(0, hq // 2)
+        assert torch.equal(out[clean], ref[clean]) and torch.equal(lse[clean], ref_lse[clean])
+        assert torch.isnan(out[hq // 2:]).all() and torch.isnan(lse[hq // 2:]).all()
+        bad_q = q.clone()
+        bad_q[0, 1, 3] = float("nan")
+        out, lse = run(k, bad_q, cap)
+        others = [h for h in range(hq) if h != 1]
+        assert torch.equal(out[others], ref[others]) and torch.equal(lse[others], ref_lse[others])
+        assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
