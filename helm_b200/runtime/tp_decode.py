@@ -257,6 +257,8 @@ class TPDecodeModel:
         """Synthetic context of `length` tokens per sequence (N(0,1) K/V)."""
         if length >= self.max_len:
             raise ValueError("context does not fit max_len")
+        if self.fp4 and self.B * -(-length // self.P) > self.free_pages.numel():
+            raise ValueError("context does not fit the pages")
         g = torch.Generator(device=self.dev).manual_seed(seed * 7919 + self.rank)
         if not self.fp4:
             self.pool.normal_(generator=g)
@@ -270,8 +272,6 @@ class TPDecodeModel:
 
         step(torch.full_like(self.lens, -1), 0)  # what they held goes back
         rows = step(torch.full_like(self.lens, length), self.B * length)
-        if _capi.device_status(self.dev) & _capi.DEV_NO_PAGES:
-            raise ValueError("context does not fit the pages")
         shape = (max(1, min(16384, rows.numel())), self.w.hkv, self.D)
         for pool in self.pools:
             k, v = (torch.randn(shape, generator=g, device=self.dev).to(self.dtype) for _ in range(2))

@@ -64,3 +64,20 @@ def test_an_idle_sequence_keeps_its_token_unless_told(dev):  # noqa: F811
     tp.step(torch.tensor([[8], [9]]))   # (what it is to start with may be given)
     assert tp.ids.view(-1).tolist() == [8, 9] and tp.lens.tolist() == [2, 0]
     tp.close()
+
+
+def test_fill_kv_and_the_device_status(dev):  # noqa: F811
+    """A refused context changes nothing; an old status neither stops fill_kv nor is lost."""
+    tp = _model(dev, num_pages=5)
+    for _ in range(49):
+        tp.step()
+    assert tp.lens.sum().item() == 80
+    before = [t.clone() for t in (tp.lens, tp.table, tp.free_pages, tp.free_count, *tp.pools)]
+    with pytest.raises(ValueError):
+        tp.fill_kv(40)   # 6 pages
+    after = (tp.lens, tp.table, tp.free_pages, tp.free_count, *tp.pools)
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+    tp.fill_kv(20)       # fits, whatever happened before
+    assert tp.lens.tolist() == [20, 20] and tp.free_count.item() == 1
+    assert _capi.device_status(dev) == _capi.DEV_NO_PAGES
+    tp.close()
