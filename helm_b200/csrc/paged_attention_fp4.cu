@@ -62,7 +62,7 @@ struct DecodeFp4Args {
   float* part_o;   // warp partials [num_workers + pairs][G][D]
   float* part_ml;  // warp partials [num_workers + pairs][G][2]
   int batch, hq, hkv, group, page_size, tiles_per_page;
-  uint32_t tpp_magic;  // x / tiles_per_page = (x * tpp_magic) >> 32 for x < 2^31 / 16, 0: shift
+  uint32_t tpp_magic;  // x / tiles_per_page = (x * tpp_magic) >> 32, 0: shift
   int tpp_shift;
   int warps;         // workers of a CTA
   int num_workers;
@@ -1025,6 +1025,13 @@ extern "C" int helm_paged_decode_attention_fp4(
   if (table_tiles >= (int64_t(1) << 30) ||
       static_cast<int64_t>(max_pages) * page_size >= (int64_t(1) << 31))
     return HELM_ERR_UNSUPPORTED;
+  // The page of tile x is (x * magic) >> 32 with magic = ceil(2^32 / tpp): the product
+  // exceeds x / tpp * 2^32 by x * over / tpp, which must stay below the 1 / tpp * 2^32
+  // that the tile before a page's end leaves.
+  const uint64_t magic = ((uint64_t(1) << 32) + tpp - 1) / tpp;
+  const uint64_t over = magic * tpp - (uint64_t(1) << 32);
+  if (static_cast<uint64_t>(max_pages) * tpp * over > (uint64_t(1) << 32))
+    return HELM_ERR_UNSUPPORTED;
   // q is read as 32-bit words, the pool with bulk copies (16-byte rule)
   if ((reinterpret_cast<uintptr_t>(q) & 3) || (q_stride_b & 1) || (q_stride_h & 1) ||
       (reinterpret_cast<uintptr_t>(kv_pool) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
@@ -1065,8 +1072,8 @@ extern "C" int helm_paged_decode_attention_fp4(
   a.tpp_shift = 0;
   if ((tpp & (tpp - 1)) == 0)
     while ((int64_t(1) << a.tpp_shift) < tpp) ++a.tpp_shift;
-  else  // rounded up: exact while x * (tpp - 1) < 2^32, and tpp * x <= 2^31 / 16 here
-    a.tpp_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + tpp - 1) / tpp);
+  else
+    a.tpp_magic = static_cast<uint32_t>(magic);
   const bool plain = mask == nullptr && !(softcap > 0.f) && scale > 0.f;
   a.score_scale = scale * k_scale;
   a.softcap = softcap;

@@ -425,7 +425,10 @@ int helm_gather_kv_rows_fp4(const void* kv_pool, int64_t pool_pages, const int64
  * contributes nothing, whatever its page holds, NaN included; a row that sees
  * no key gets O = 0, LSE = -inf.  q: 4-byte aligned, even strides.  mask_len:
  * values in a row of the mask; a length beyond it, or beyond the page table's
- * row, is cut and HELM_DEV_BAD_PAGE recorded.
+ * row, is cut and HELM_DEV_BAD_PAGE recorded.  Tables of 2^31 tokens a sequence or
+ * 2^30 tiles in all are not supported, nor (page sizes that are no power of two)
+ * those whose page numbers a 32-bit reciprocal does not give exactly: 1.1e9
+ * tokens a sequence with pages of 1008, 1.7e7 with pages of 65552.
  *  workspace  >= helm_paged_decode_fp4_workspace_bytes(...) bytes, 256-byte
  *             aligned, any contents; calls that overlap on the GPU need one each
  */
