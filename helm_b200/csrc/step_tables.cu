@@ -331,8 +331,10 @@ extern "C" int helm_build_step_tables(const int32_t* past_lens, const int32_t* n
       pt_stride_b < max_pages)
     return HELM_ERR_INVALID_ARGUMENT;
   if (batch > kStepMaxRequests) return HELM_ERR_UNSUPPORTED;
-  // page counts of all requests together, and positions, are 32-bit
-  if (static_cast<int64_t>(batch) * max_pages >= (int64_t(1) << 31) ||
+  // positions are 32-bit; so are the counts of pages and tokens, and a stride of the
+  // whole cluster beyond them
+  if (static_cast<int64_t>(batch) * max_pages > (int64_t(1) << 30) ||
+      num_rows > (int64_t(1) << 30) ||
       static_cast<int64_t>(max_pages) * page_size >= (int64_t(1) << 31))
     return HELM_ERR_UNSUPPORTED;
   int shift = -1;

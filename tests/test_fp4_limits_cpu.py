@@ -2,7 +2,7 @@
 leave its range are refused (no GPU needed)."""
 import pytest
 
-from test_fp4_cpu import ALIGN, P16, UNSUPPORTED, _decode
+from test_fp4_cpu import ALIGN, P16, UNSUPPORTED, _decode, _tables
 
 WIDE = dict(batch=1, hq=1, hkv=1, q=P16 + 2)   # what is not refused goes on to the alignment
 
@@ -46,3 +46,10 @@ def test_wrong_page_numbers_exist():
     assert (x * _reciprocal(4097)) >> 32 != x // 4097
     assert _decode(page=65552, maxp=274, pt_sb=274, **WIDE) == UNSUPPORTED
     assert _decode(page=65552, maxp=250, pt_sb=250, **WIDE) == ALIGN
+
+
+def test_step_tables_whose_loops_would_pass_32_bits():
+    """Threads step through rows and pages in strides of 16 * 1024 * 4."""
+    for n in (2 ** 31 - 1, 2 ** 31 - 65536, 2 ** 30 + 1):
+        assert _tables(n=n) == UNSUPPORTED
+    assert _tables(batch=8191, maxp=1 << 18, sb=1 << 18, page=16) == UNSUPPORTED
