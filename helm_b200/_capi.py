@@ -973,6 +973,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
         if t is not None and (t.dtype is not dt or t.shape != each or not t.is_contiguous()):
             _refuse(what, "uniforms, temperature, top_p, min_p and logprobs must be contiguous fp32 "
                           "[B], top_k int32 [B], out int64 [B]")
+    if B == 0:  # (empty tensors have no address)
+        return out
     rc = _call(idx, (_lib or lib()).helm_sample_tokens, logits.data_ptr(), ls[0],
                helm_dtype(logits.dtype), uniforms.data_ptr(), _ptr(temperature), _ptr(top_k),
                _ptr(top_p), _ptr(min_p), out.data_ptr(), _ptr(logprobs), B, V,

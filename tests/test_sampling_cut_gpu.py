@@ -21,3 +21,9 @@ def test_shares_that_end_on_a_border_of_fp32_sums(dev, seed):  # noqa: F811
     _check(dev, x, u, top_p=p)
     _check(dev, x, u, top_p=p, top_k=np.where(np.arange(len(p)) % 2, 0, 150000))
     assert _capi.device_status(dev) == 0
+
+
+def test_no_rows(dev):  # noqa: F811
+    x, u = torch.empty(0, 100, device=dev), torch.empty(0, device=dev)
+    ids = _capi.sample_tokens(x, u, logprobs=torch.empty(0, device=dev))
+    assert ids.shape == (0,) and ids.dtype == torch.int64
