@@ -700,6 +700,18 @@ def _stream_of(idx: int, stream) -> int:
     return torch.cuda.current_stream(idx).cuda_stream
 
 
+def _empty(shape, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    """Memory that a call on `stream` (None: the current one) writes.  It comes from
+    that stream's own: a block that the current stream has freed may still be in use
+    by what is queued there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))  # the caller may use it there
+    return t
+
+
 def _check_fp4_pool(what: str, pool: torch.Tensor, hkv: int, page_size: int, d: int) -> None:
     shape = pool.shape
     if (pool.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != hkv
@@ -782,13 +794,9 @@ def gather_kv_rows_fp4(pool: torch.Tensor, slot_rows: torch.Tensor, *, page_size
         _refuse(what, "slot_rows must be contiguous int64 [N]")
     N = slot_rows.shape[0]
     if k_out is None:
-        k_out = torch.empty((N, Hkv, D), dtype=dtype, device=pool.device)
-        if stream is not None:
-            k_out.record_stream(stream)
+        k_out = _empty((N, Hkv, D), dtype, pool.device, stream)
     if v_out is None:
-        v_out = torch.empty((N, Hkv, D), dtype=dtype, device=pool.device)
-        if stream is not None:
-            v_out.record_stream(stream)
+        v_out = _empty((N, Hkv, D), dtype, pool.device, stream)
     ks, vs, shape = k_out.stride(), v_out.stride(), (N, Hkv, D)
     if (k_out.shape != shape or v_out.shape != shape or k_out.dtype is not dtype
             or v_out.dtype is not dtype or ks[2] != 1 or vs[2] != 1):
@@ -838,9 +846,7 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
     if kv_lens.dtype is not i32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
         _refuse(what, "kv_lens must be contiguous int32 [B]")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=q.device)
-        if stream is not None:
-            out.record_stream(stream)
+        out = _empty(shape, dt, q.device, stream)
     os_ = out.stride()
     if out.dtype is not dt or out.shape != shape or os_[2] != 1:
         _refuse(what, "out must be [B, Hq, D] in the query dtype, unit dim stride")
@@ -866,9 +872,7 @@ def paged_decode_attention_fp4(q: torch.Tensor, pool: torch.Tensor, page_table: 
         nbytes = _fp4_ws_bytes[key] = int(
             _call(idx, L.helm_paged_decode_fp4_workspace_bytes, B, Hq, num_kv_heads, D))
     # scratch of this call alone: two captured graphs, or two streams, share none
-    ws = pool.new_empty(nbytes)
-    if stream is not None:
-        ws.record_stream(stream)
+    ws = pool.new_empty(nbytes) if stream is None else _empty(nbytes, torch.uint8, pool.device, stream)
     rc = _call(idx, L.helm_paged_decode_attention_fp4, q.data_ptr(), qs[0], qs[1], pool.data_ptr(),
                pool.shape[0], page_table.data_ptr(), ts[0], tshape[1], kv_lens.data_ptr(),
                mask_ptr, mask_dt, mask_sb, mask_len, out.data_ptr(), os_[0], os_[1], lse_ptr,
@@ -903,23 +907,19 @@ def build_step_tables(past_lens: torch.Tensor, new_lens: torch.Tensor, page_tabl
     if past_lens.dtype is not i32 or past_lens.dim() != 1:
         _refuse(what, "past_lens must be int32 [B]")
     B = past_lens.shape[0]
-    new = past_lens.new_empty
+    dev = past_lens.device
     if free_count_out is None:
         free_count_out = free_count
-    made = []  # what this call allocates
     if kv_lens is None:
-        made.append(kv_lens := new(B))
+        kv_lens = _empty(B, i32, dev, stream)
     if cu_tokens is None:
-        made.append(cu_tokens := new(B + 1))
+        cu_tokens = _empty(B + 1, i32, dev, stream)
     if seq_ids is None:
-        made.append(seq_ids := new(num_rows))
+        seq_ids = _empty(num_rows, i32, dev, stream)
     if positions is None:
-        made.append(positions := new(num_rows))
+        positions = _empty(num_rows, i32, dev, stream)
     if slot_rows is None:
-        made.append(slot_rows := new(num_rows, dtype=torch.int64))
-    if stream is not None:
-        for t in made:
-            t.record_stream(stream)
+        slot_rows = _empty(num_rows, torch.int64, dev, stream)
     _same_device(what, idx, new_lens, page_table, free_pages, free_count, free_count_out, kv_lens,
                  cu_tokens, seq_ids, positions, slot_rows)
     one, each, rows = (1,), (B,), (num_rows,)
@@ -964,9 +964,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
         _refuse(what, "logits must be [B, V] with a unit inner stride")
     B, V = shape
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=logits.device)
-        if stream is not None:
-            out.record_stream(stream)
+        out = _empty(B, torch.int64, logits.device, stream)
     f32, each = torch.float32, (B,)
     for t, dt in ((uniforms, f32), (temperature, f32), (top_k, torch.int32), (top_p, f32),
                   (min_p, f32), (out, torch.int64), (logprobs, f32)):
