@@ -11,8 +11,10 @@
 // kernel is built around few instructions per value:
 //   * cvt.rn.f16x2.e2m1x2 widens two values, one HMUL2 applies their scale
 //     (exact: see fp4.cuh); both matrix products run as fp16 mma.sync m16n8k16
-//     with fp32 accumulation.  tcgen05 would need the widened tile written
-//     back to shared memory for its operand, more work than the product itself.
+//     with fp32 accumulation.  tcgen05's fp16 kind would need the widened tile
+//     written back to shared memory for its operand, more work than the product
+//     itself; its block-scaled FP4 kind takes K as it lies, but wants q as a sum of
+//     FP4 numbers, and has no place for V, whose blocks run along the other axis.
 //   * The reduction index of a product may be taken in any order, so a lane
 //     reads 16 contiguous bytes of a K row (32 dims) as its A fragments of all
 //     eight k-steps, and a V chunk's dims as its rows of all m-tiles; the
@@ -105,8 +107,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// tanh without a branch: its odd series to x^11 below 1/4 (next term 2e-10), else
-// 1 - 2 / (e^2x + 1) (3e-7 absolute).
+// tanh without a branch: its Taylor series to x^11 below 1/4 (next term 2e-10), else
+// the identity 1 - 2 / (e^2x + 1) (3e-7 absolute).
 __device__ __forceinline__ float tanh_fast(float x) {
   const float z = x * x;
   float p = fmaf(z, -1382.f / 155925.f, 62.f / 2835.f);
@@ -950,7 +952,7 @@ template <typename T, int D>
 cudaError_t dispatch_decode_fp4_nt(const DecodeFp4Args& a, bool plain, int64_t units,
                                    cudaStream_t s) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  if (kHalf && a.group <= 4)  // 16 x 2k tokens, one head a KV head: 50.4 us, two products 53.9
+  if (kHalf && a.group <= 4)  // 16 x 2k tokens, one head a KV head: 50.2 us, two products 53.9
     return plain ? launch_decode_fp4<T, D, 1, true, kHalf>(a, units, s)
                  : launch_decode_fp4<T, D, 1, false, kHalf>(a, units, s);
   if (a.group <= 8)

@@ -19,9 +19,11 @@
 // With few rows a row is held by one cluster, its logits in the CTAs' shared
 // memory.  With at least as many rows as SMs one CTA does a row, reading it from
 // L2 once per pass: no cluster barriers, and two rows share an SM, one computing
-// while the other waits (256 x 151936 bf16: top-k 144 -> 94 us, no filter 127 ->
-// 93).  Bound by instructions: some 30 per logit for its weight, 10 for a bin; a
-// long bf16 row looks its weights up in a table of its possible values instead.
+// while the other waits (256 x 151936 bf16, every filter mixed: 184 -> 118 us).
+// Bound by instructions: some 30 per logit for its weight, 10 for a bin; a long bf16
+// row looks its weights up in a table of its possible values instead.  A call also
+// waits for its heaviest rows, each one CTA from start to end: 256 rows of top-p
+// alone take 137 us, of top-k alone 78, without a filter 80.
 //
 // A filter needs its last kept candidate.  A histogram of counts over 2048 equal
 // steps of the logit (equal steps spread a bell-shaped row over the bins; digits
@@ -67,7 +69,7 @@ constexpr int kSampMaxCluster = 8;
 // entry for what lies beyond.
 constexpr int kSampLutSide = 2048 + 1;
 constexpr int kSampLutBytes = 2 * kSampLutSide * (8 + 4);  // weights and counts
-constexpr int kSampLutLogits = 65536;  // of a CTA, from which the table pays
+constexpr int kSampLutLogits = 65536;  // of a row that has the table (launch_sample says why)
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -110,7 +112,8 @@ __device__ const double kExp2Table[64] = {
     0x1.fa7c1819e90d8p+0,
 };
 
-// w = exp(x) in units of 2^-44 for -31.4 < x <= 0, given y = x * 64 / ln 2:
+// w = exp(x) in units of 2^-44 for -31.4 < x <= 0, given y = x * 64 / ln 2, by Tang's
+// table-driven method (ACM Trans. Math. Softw. 15, 1989) with a Taylor tail:
 // 2^(j/64) from the table, e^r = 2^(y/64 - k/64) by its series to the fourth
 // power (|r| <= ln2/128, next term < 4e-14), rounded to nearest by adding 2^52.
 // No branches: the caller's loop interleaves several of these chains, which is
@@ -569,7 +572,7 @@ struct Sampler {
   // by value, and counts times weights, taken in the order of the values, say
   // exactly in which value each filter ends and how many of its candidates, in
   // index order, are kept.  One more pass sums what is kept and finds the last of
-  // those.  (256 x 151936, top-p: 210 us without it, 138 with.)  False where a filter
+  // those.  (256 x 151936, top-p: 212 us without it, 137 with.)  False where a filter
   // ends among the values below the table, which are counted as one.
   static constexpr int kLutPos = 2 * kSampLutSide + 1;  // positive, below the table, negative
   static constexpr int kLutPer = (kLutPos + kSampThreads - 1) / kSampThreads;
@@ -1260,7 +1263,10 @@ cudaError_t launch_sample(SampleArgs a, int batch, int ctas, cudaStream_t stream
   a.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
   // The table of weights costs 4098 of them: slower with the slices of a cluster
   // (64 x 151936 in slices of 19k: 66.8 -> 69.8 us), faster with whole rows (256 x
-  // 151936, no filter: 93 -> 81, top-k 95 -> 79, top-p with by_value 220 -> 138).
+  // 151936, no filter: 104 -> 80, top-k 103 -> 78, top-p with by_value 234 -> 137; at
+  // 65536 logits 46 -> 38, mixed filters 86 -> 58).  Shorter whole rows would gain as
+  // well (16384 logits: no filter 19.9 -> 18.8, mixed 40 -> 28); they share the path of
+  // fp16 and fp32 rows.
   a.tabled = !kResident && std::is_same<T, __nv_bfloat16>::value && a.vocab >= kSampLutLogits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));
@@ -1282,6 +1288,11 @@ template <typename T>
 cudaError_t dispatch_sample(const SampleArgs& a, int batch, cudaStream_t stream) {
   const int sms = num_sms_current_device();
   constexpr int kVec = 16 / sizeof(T);
+  // Whole rows from L2 or clusters, mixed filters, us: 151936 bf16 at 74 rows 92 / 71,
+  // 120: 94 / 100, 148: 97 / 121, 256: 118 / 184; fp32 at 120: 143 / 130, 148: 145 / 161,
+  // 256: 182 / 261; fp16 (no table) at 148: 139 / 122, 200: 170 / 147, 256: 170 / 182.
+  // 32000 bf16 and fp16: within a tenth from 120 rows on; fp32 at 148: 43 / 38, 200: 49
+  // / 56.
   if (batch >= sms && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
       a.row_stride % kVec == 0 && a.vocab % kVec == 0)
     return launch_sample<T, false>(a, batch, 1, stream);

@@ -4,7 +4,8 @@ HELM's PipelineRuntime decodes greedily (helm/runtime/pipeline_runtime.py:300-33
 argmax, eos / pad handling); greedy stays the default here.  With SamplingParams
 the loops draw the token on the device instead (helm_sample_tokens): temperature,
 top-k, top-p and min-p, from uniforms that a seeded generator on the host gives,
-so the same seed gives the same tokens eagerly and from a replayed graph.
+so the same seed gives the same tokens eagerly and from a replayed graph.  Vocabularies
+of up to 262144 tokens.
 """
 from __future__ import annotations
 

@@ -489,7 +489,8 @@ int helm_build_step_tables(const int32_t* past_lens, const int32_t* new_lens, in
  *  top_k       [batch] int32 (NULL, <= 0 or >= vocab: all): the first k
  *  top_p       [batch] fp32 (NULL or >= 1: all): of those, the shortest prefix
  *              whose weights reach top_p of their sum (one candidate at least)
- *  min_p       [batch] fp32 (NULL or <= 0: all): w_i >= min_p
+ *  min_p       [batch] fp32 (NULL or <= 0: all; above 1: as 1): w_i >= min_p, so
+ *              every candidate that equals the largest stays
  *  uniforms    [batch] fp32 in [0, 1): the token is the smallest index whose
  *              running sum of kept weights, in index order, exceeds u * their sum
  *  ids         [batch] int64 out; -1 for a row without a candidate above -inf
