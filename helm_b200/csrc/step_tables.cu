@@ -331,10 +331,11 @@ extern "C" int helm_build_step_tables(const int32_t* past_lens, const int32_t* n
       pt_stride_b < max_pages)
     return HELM_ERR_INVALID_ARGUMENT;
   if (batch > kStepMaxRequests) return HELM_ERR_UNSUPPORTED;
-  // positions are 32-bit; so are the counts of pages and tokens, and a stride of the
-  // whole cluster beyond them
-  if (static_cast<int64_t>(batch) * max_pages > (int64_t(1) << 30) ||
-      num_rows > (int64_t(1) << 30) ||
+  // positions are 32-bit; so are the counts of pages and tokens, and a stride of all
+  // threads beyond them
+  static_assert(kStepCluster * kStepThreads * std::max(kStepRun, kStepTokens) < 1 << 17, "");
+  constexpr int64_t kMost = (int64_t(1) << 31) - (1 << 17);
+  if (static_cast<int64_t>(batch) * max_pages > kMost || num_rows > kMost ||
       static_cast<int64_t>(max_pages) * page_size >= (int64_t(1) << 31))
     return HELM_ERR_UNSUPPORTED;
   int shift = -1;

@@ -468,8 +468,8 @@ int helm_paged_decode_attention_fp4(const void* q, int64_t q_stride_b, int64_t q
  * included) exceed the free ones: its length and pages stay, its tokens' rows
  * are -1, and HELM_DEV_NO_PAGES is recorded.  free_count_out apart, a repeated
  * call with the same inputs gives the same outputs.  B <= 8192; B * max_pages
- * and num_rows at most 2^30; max_pages * page_size and the sum of new_lens below
- * 2^31 (a larger sum saturates).
+ * and num_rows at most 2^31 - 2^17; max_pages * page_size and the sum of
+ * new_lens below 2^31 (a larger sum saturates).
  *
  * Replaces the host bookkeeping of KVAllocator.allocate / free
  * (helm/runtime/kv_allocator.py:36-93) where a step runs without the host.

@@ -50,6 +50,8 @@ def test_wrong_page_numbers_exist():
 
 def test_step_tables_whose_loops_would_pass_32_bits():
     """Threads step through rows and pages in strides of 16 * 1024 * 4."""
-    for n in (2 ** 31 - 1, 2 ** 31 - 65536, 2 ** 30 + 1):
+    most = 2 ** 31 - 2 ** 17
+    for n in (2 ** 31 - 1, 2 ** 31 - 65536, most + 1):
         assert _tables(n=n) == UNSUPPORTED
-    assert _tables(batch=8191, maxp=1 << 18, sb=1 << 18, page=16) == UNSUPPORTED
+    wide = most // 4096
+    assert _tables(batch=4096, maxp=wide + 1, sb=wide + 1, page=16) == UNSUPPORTED
